@@ -121,6 +121,35 @@ typedef struct tp_server tp_server;
  *   p: x,pre_gamma,pre_beta|0,pre_mean|0,pre_var|0,w,y,post_gamma|0,post_beta|0,post_mean|0,post_var|0[,residual|0]
  *   i: rows,cin,cout,x_pitch,y_pitch,pre_relu,act   f: pre_eps,post_eps */
 #define TP_OP_BN_CONV1X1 18
+/* The three operators of an encoder layer in 8 bits.  An int8 row holds codes q in -127 .. 127 and one float scale s; it
+ * stands for s * q.  All are per row: a row's results do not depend on the other rows, on the number of rows or on
+ * the kernel variant.  Pitches are in elements, 0 = dense; no operand needs more than its element's alignment.  Bytes
+ * between a row's end and the next row are neither read nor written.  rows = 0 (m or n = 0) is a call that does nothing.
+ *
+ * Rows of floats to int8 rows.  amax = the row's largest magnitude, s = max(amax / 127, 2^-126) rounded to float, q the
+ * integer nearest to x / s, halves to even.  A row that holds an infinity or a NaN gets s = NaN and q = 0.
+ * width up to 65536 (TP_EUNSUPPORTED beyond).  q and scale must not overlap x.
+ *   p: x,q,scale   i: rows,width[,x_pitch,q_pitch] */
+#define TP_OP_QUANT_ROWS 19
+/* Matrix product of int8 rows: y[r][c] = act(x_scale[r] * w_scale[c] * sum_k x[r][k] * w[c][k] + bias[c] + residual[r][c]).
+ * The sum is exact (int32; k up to 131071, TP_EUNSUPPORTED beyond), then rounded to float and scaled in float.  Codes may
+ * also be -128.  k = 0 gives act(bias + residual).  residual may be y itself with the same pitch; y overlaps nothing else.
+ *   p: x,x_scale,w,w_scale,y[,bias|0,residual|0]   i: m,n,k[,x_pitch,w_pitch,y_pitch,residual_pitch,act]   (0 = k,k,n,n) */
+#define TP_OP_GEMM_I8 20
+/* The norms around a block, its gate and the residual stream, in one pass:
+ *   t = x, or norm_post(x) * post_gamma + post_beta
+ *   h = residual_scale * residual + block_scale * gate * t                 rounded to float
+ *   y = h, or norm_pre(h) * pre_gamma + pre_beta                           rounded to float
+ *   q, scale = y as int8 rows (as TP_OP_QUANT_ROWS)
+ * post / pre: 0 = none, 1 = layer norm (v - mean) / sqrt(var + eps), 2 = root mean square norm v / sqrt(mean(v^2) + eps).
+ * A norm needs its gamma; its beta is optional, and both are 0 without the norm.  gate: one row of `width` values for
+ * every row of x (rows_per_gate = 0), or row r / rows_per_gate of it.  Outputs h, y and the pair q, scale are optional, one
+ * of them must be given.  h and y may be x or residual themselves (same pitch); outputs overlap nothing else.  Statistics and
+ * arithmetic are in double: calls that split the chain after h or y compute the same bits.  width up to 65536.
+ *   p: x,residual|0,gate|0,post_gamma|0,post_beta|0,pre_gamma|0,pre_beta|0,h|0,y|0[,q|0,scale|0]
+ *   i: rows,width,post,pre[,rows_per_gate,x_pitch,residual_pitch,h_pitch,y_pitch,q_pitch]
+ *   f: residual_scale,block_scale,post_eps,pre_eps */
+#define TP_OP_NORM_BLOCK 21
 
 typedef struct tp_config {
     uint32_t struct_size;       /* sizeof(tp_config) */
@@ -337,6 +366,14 @@ int tp_bn_inference_pitched(tp_server* s, int32_t client, uint64_t x, uint64_t y
  *     after such an event the process must not go on using this entry point. */
 #define TP_NOALLOC_SCRATCH_BYTES (16u << 20)
 int tp_gemm_noalloc(const tp_gemm_desc* d, void* stream);
+/* tp_launch for the same callers: the argument lists are tp_launch's, with raw device addresses of the current HIP
+ * device, enqueued on `stream` of that device.  Takes TP_OP_QUANT_ROWS, TP_OP_GEMM_I8 and TP_OP_NORM_BLOCK
+ * (TP_EUNSUPPORTED for the others), which use no scratch memory at all: calls on different streams and captured graphs may
+ * overlap freely, and results are bit-identical to tp_launch's.  Arguments are checked as there, except that nothing is
+ * known about how large the caller's buffers are.  The first call on each GPU may load the library's code object: make it
+ * outside graph capture. */
+int tp_launch_noalloc(int32_t op_id, const uint64_t* ptrs, int32_t n_ptrs, const int64_t* ints, int32_t n_ints,
+                      const float* floats, int32_t n_floats, void* stream);
 /* cudaLaunchKernelService (cuda_server.hpp:1226-1310) by op id, pointer slots explicit. */
 int tp_launch(tp_server* s, int32_t client, int32_t op_id, const uint64_t* ptrs, int32_t n_ptrs,
               const int64_t* ints, int32_t n_ints, const float* floats, int32_t n_floats);

@@ -191,3 +191,58 @@ def embedding(ids, type_ids, word, pos, typ, seq):
     y = np.empty((ids.size, width), np.float32)
     lib().ref_embedding(_p(ids), _p(tids), _p(word), _p(pos), _p(typ), _p(y), C.c_long(ids.size), seq, width)
     return y
+
+
+def quant_rows(x):
+    """Rows of float32 to int8 codes and one float32 scale a row: amax / 127 rounded to float32, at least 2^-126; the code is the
+    integer nearest to the quotient by that scale, halves to even.  In float64 the quotient of two float32 numbers
+    that is not itself a half never rounds to one, so numpy's rint of it is the rounding of the true quotient.  A row
+    with an infinity or a NaN: scale NaN, codes 0."""
+    x = np.asarray(x, np.float32).astype(np.float64)
+    with np.errstate(invalid="ignore"):
+        amax = np.abs(x).max(1)
+        bad = ~np.isfinite(x).all(1)
+        scale = np.maximum((amax / 127.0).astype(np.float32), np.float32(2.0 ** -126))
+        scale[bad] = np.float32("nan")
+        q = np.rint(x / scale.astype(np.float64)[:, None])
+    q[bad] = 0
+    return q.astype(np.int8), scale
+
+
+def gemm_i8(xq, sx, wq, sw, bias=None, residual=None, act="none"):
+    """act(sx[r] sw[c] sum_k xq[r,k] wq[c,k] + bias[c] + residual[r,c]) in float64, and what the sum before `act` is."""
+    from scipy.special import erf, expit
+
+    s = np.asarray(xq, np.int64).astype(np.float64) @ np.asarray(wq, np.int64).astype(np.float64).T   # exact below 2^53
+    v = s * np.asarray(sx, np.float64)[:, None] * np.asarray(sw, np.float64)[None, :]
+    if bias is not None:
+        v = v + np.asarray(bias, np.float64)
+    if residual is not None:
+        v = v + np.asarray(residual, np.float64)
+    y = {"none": lambda t: t, "relu": lambda t: np.maximum(t, 0.0), "gelu": lambda t: 0.5 * t * (1.0 + erf(t / np.sqrt(2.0))),
+         "tanh": np.tanh, "relu6": lambda t: np.clip(t, 0.0, 6.0), "silu": lambda t: t * expit(t), "sigmoid": expit}[act](v)
+    return y, v
+
+
+def norm_block(x, residual=None, gate=None, rows_per_gate=0, post=None, pre=None, a=1.0, b=1.0):
+    """The norms around a block in float64.  post / pre: None or (kind, gamma, beta or None, eps).  Returns (h, y): h as it is before
+    its rounding to float32, y of the rounded h."""
+    def norm(t, kind, gamma, beta, eps):
+        if kind == "layer":
+            t = t - t.mean(1, keepdims=True)
+        t = t / np.sqrt((t * t).mean(1, keepdims=True) + eps) * np.asarray(gamma, np.float64)
+        return t if beta is None else t + np.asarray(beta, np.float64)
+
+    t = np.asarray(x, np.float64)
+    if post is not None:
+        t = norm(t, *post)
+    if gate is not None:
+        g = np.atleast_2d(np.asarray(gate, np.float64))
+        t = t * (g[np.arange(t.shape[0]) // rows_per_gate] if rows_per_gate else g)
+    t = t * b
+    if residual is not None:
+        t = t + a * np.asarray(residual, np.float64)
+    y = t.astype(np.float32).astype(np.float64)
+    if pre is not None:
+        y = norm(y, *pre)
+    return t, y

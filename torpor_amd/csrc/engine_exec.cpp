@@ -1,4 +1,5 @@
 #include "engine_internal.hpp"
+#include "layer_ops.hpp"
 
 namespace tp {
 
@@ -63,7 +64,8 @@ int Engine::exec_compute_impl(Model& m, const Op& op, bool launch) {
         /* MAXPOOL */ 1u << 8, /* AVGPOOL */ 0, /* LAYERNORM */ 1u << 0, /* SOFTMAX */ (1u << 0) | (1u << 2),
         /* EMBEDDING */ (1u << 0) | (1u << 3), /* NCHW_TO_NHWC */ 0, /* NHWC_TO_NCHW */ 0, /* SUM */ 1u << 0,
         /* FILL */ 1u << 0, /* ATTENTION */ 0xF0u, /* AVGPOOL2D */ 1u << 7, /* COPY2D */ (1u << 0) | (1u << 2) | (1u << 3),
-        /* SCALE_CHANNELS */ 1u << 1, /* BN_CONV1X1 */ (1u << 0) | (1u << 3) | (1u << 4)};
+        /* SCALE_CHANNELS */ 1u << 1, /* BN_CONV1X1 */ (1u << 0) | (1u << 3) | (1u << 4),
+        /* QUANT_ROWS */ 0xDu, /* GEMM_I8 */ 0x78u, /* NORM_BLOCK */ 0x3F1u};
     {
         uint32_t long_mask = 0;
         switch (op.kind) {
@@ -361,6 +363,19 @@ int Engine::exec_compute_impl(Model& m, const Op& op, bool launch) {
             return tpk::launch_attention(F(0), F(1), F(2), F(3), Fm(4), (int)B, (int)A, (int)S, (int)dh, I[4], I[5],
                                          I[6], I[7], op.f[0], compute_);
         }
+        case TP_OP_QUANT_ROWS:
+        case TP_OP_GEMM_I8:
+        case TP_OP_NORM_BLOCK: {
+            Operands list;
+            if ((r = layer_op_operands(op.op_id, op.p, op.np, op.i, op.ni, op.nf, &list))) return r;
+            for (int k = 0; k < list.n; ++k) {
+                const Operand& o = list.v[k];
+                if ((r = R(o.slot, false, o.span(), o.elem))) return r;
+            }
+            if (layer_op_overlap(list)) return TP_EINVAL;
+            if (!launch || list.empty) return 0;
+            return layer_op_launch(op.op_id, q, op.i, op.ni, op.f, compute_);
+        }
         case TP_OP_FILL:
             if (!need(1, 1, 1)) return TP_EINVAL;
             if ((r = R(0, false, I[0]))) return r;
@@ -431,6 +446,22 @@ void op_work(const Op& op, double* flops, double* bytes, const char** name) {
                     *flops = 4.0 * (double)(I[0] * I[1]) * (double)(I[2] * I[2]) * (double)I[3];
                     *bytes = 16.0 * (double)(I[0] * I[2]) * (double)(I[1] * I[3]);
                     *name = "attention";
+                    break;
+                case TP_OP_QUANT_ROWS:
+                    *bytes = 5.0 * (double)I[0] * (double)I[1];
+                    *name = "quant_rows";
+                    break;
+                case TP_OP_GEMM_I8: {
+                    const double m = (double)I[0], n = (double)I[1], k = (double)I[2];
+                    *flops = 2.0 * m * n * k;
+                    *bytes = (m + n) * (k + 4.0) + 4.0 * m * n * (op.p[6] ? 2.0 : 1.0);
+                    *name = "gemm_i8";
+                    break;
+                }
+                case TP_OP_NORM_BLOCK:
+                    *bytes = (double)I[0] * (double)I[1] *
+                             (4.0 + (op.p[1] ? 4.0 : 0.0) + (op.p[7] ? 4.0 : 0.0) + (op.p[8] ? 4.0 : 0.0) + (op.p[9] ? 1.0 : 0.0));
+                    *name = "norm_block";
                     break;
                 default: break;
             }

@@ -122,6 +122,49 @@ int launch_softmax(const float* x, const float* mask, float* y, long rows, int w
 // operand is at pointer + (b*S + t)*ld, head a at column a*dh.  dh must be 64.
 int launch_attention(const float* q, const float* k, const float* v, const float* mask, float* out, int B, int A, int S,
                      int dh, long ldq, long ldk, long ldv, long ldo, float scale, hipStream_t s);
+
+// ---- 8-bit encoder layer (int8_rows.hip, gemm_i8.hip).  Pitches in elements, any alignment, no scratch memory. ----
+constexpr int kRowOpMaxWidth = 65536;  // a row lives in the registers of one workgroup
+constexpr int kGemmI8MaxK = 131071;    // |sum| <= k * 128 * 128 stays below 2^31
+struct QuantRowsArgs {
+    const float* x = nullptr;
+    int8_t* q = nullptr;
+    float* scale = nullptr;
+    long rows = 0;
+    int width = 0;
+    long ldx = 0, ldq = 0;
+};
+// scale[r] = max(max|x[r]| / 127, 2^-126), q = x / scale to the nearest integer, halves to even
+int launch_quant_rows(const QuantRowsArgs& a, hipStream_t s);
+struct GemmI8Args {
+    const int8_t* x = nullptr;  // [m][ldx]
+    const float* sx = nullptr;  // [m]
+    const int8_t* w = nullptr;  // [n][ldw]
+    const float* sw = nullptr;  // [n]
+    float* y = nullptr;         // [m][ldy]
+    const float* bias = nullptr;
+    const float* residual = nullptr;  // [m][ldr]
+    int m = 0, n = 0, k = 0;
+    long ldx = 0, ldw = 0, ldy = 0, ldr = 0;
+    int act = 0;
+};
+// y = act(sx[r] * sw[c] * sum_k x[r][k] * w[c][k] + bias[c] + residual[r][c])
+int launch_gemm_i8(const GemmI8Args& a, hipStream_t s);
+struct NormBlockArgs {
+    const float *x = nullptr, *residual = nullptr, *gate = nullptr;
+    const float *post_gamma = nullptr, *post_beta = nullptr, *pre_gamma = nullptr, *pre_beta = nullptr;
+    float *h = nullptr, *y = nullptr;
+    int8_t* q = nullptr;
+    float* scale = nullptr;
+    long rows = 0;
+    int width = 0;
+    int post = 0, pre = 0;   // 0 none, 1 layer norm, 2 root mean square
+    long rows_per_gate = 0;  // 0: one gate row for all
+    long ldx = 0, ldr = 0, ldh = 0, ldy = 0, ldq = 0;
+    float residual_scale = 1.f, block_scale = 1.f, post_eps = 0.f, pre_eps = 0.f;
+};
+// h = residual_scale * residual + block_scale * gate * norm_post(x);  y = norm_pre(h);  q, scale = quantised rows of y
+int launch_norm_block(const NormBlockArgs& a, hipStream_t s);
 int launch_embedding(const int64_t* ids, const int64_t* type_ids, const float* word, const float* pos,
                      const float* type, float* y, long tokens, int seq, int width, long vocab, int n_types,
                      hipStream_t s);

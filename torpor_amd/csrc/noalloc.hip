@@ -1,4 +1,5 @@
-// tp_gemm_noalloc: the GEMM of tp_gemm for callers that must not allocate (code under HIP graph
+// tp_gemm_noalloc (and, at the end, tp_launch_noalloc, which needs none of what follows):
+// the GEMM of tp_gemm for callers that must not allocate (code under HIP graph
 // capture, tight serving loops, harnesses that forbid hipMalloc).  It takes raw device addresses
 // instead of an engine's virtual ones, runs on the caller's stream and keeps the only scratch memory
 // the GEMM kernels use -- the partial sums of a K range split over workgroups -- in a fixed array
@@ -15,6 +16,7 @@
 
 #include "../../include/torpor_amd.h"
 #include "kernels/kernels.hpp"
+#include "layer_ops.hpp"
 
 namespace {
 
@@ -112,4 +114,18 @@ extern "C" int tp_gemm_noalloc(const tp_gemm_desc* d, void* stream) {
     // loaded and every launch leaves them zero, so nothing has to be cleared between calls.
     const tpk::Workspace ws{ptr + kTicketBytes / 4, kScratchBytes - kTicketBytes, nullptr, reinterpret_cast<unsigned*>(ptr)};
     return tpk::launch_gemm(g, ws, static_cast<hipStream_t>(stream));
+}
+
+// tp_launch for the operators that use no scratch memory.
+extern "C" int tp_launch_noalloc(int32_t op_id, const uint64_t* ptrs, int32_t n_ptrs, const int64_t* ints, int32_t n_ints,
+                                 const float* floats, int32_t n_floats, void* stream) {
+    if (n_ptrs < 0 || n_ptrs > 12 || n_ints < 0 || n_ints > 20 || n_floats < 0 || n_floats > 4) return TP_EINVAL;
+    if ((n_ptrs && !ptrs) || (n_ints && !ints) || (n_floats && !floats)) return TP_EINVAL;
+    tp::Operands list;
+    const int r = tp::layer_op_operands(op_id, ptrs, n_ptrs, ints, n_ints, n_floats, &list);
+    if (r || list.empty) return r;
+    if (tp::layer_op_overlap(list)) return TP_EINVAL;
+    void* q[12] = {nullptr};
+    for (int k = 0; k < n_ptrs; ++k) q[k] = reinterpret_cast<void*>(static_cast<uintptr_t>(ptrs[k]));
+    return tp::layer_op_launch(op_id, q, ints, n_ints, floats, static_cast<hipStream_t>(stream));
 }

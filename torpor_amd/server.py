@@ -19,7 +19,8 @@ ACT_NONE, ACT_RELU, ACT_GELU, ACT_TANH, ACT_RELU6, ACT_SILU, ACT_SIGMOID = 0, 1,
 NCHW, NHWC = 0, 1
 (OP_RELU, OP_ADD, OP_BIAS_ACT, OP_GELU, OP_MAXPOOL, OP_AVGPOOL, OP_LAYERNORM, OP_SOFTMAX, OP_EMBEDDING,
  OP_NCHW_TO_NHWC, OP_NHWC_TO_NCHW, OP_SUM, OP_FILL, OP_ATTENTION, OP_AVGPOOL2D, OP_COPY2D,
- OP_SCALE_CHANNELS, OP_BN_CONV1X1) = range(1, 19)
+ OP_SCALE_CHANNELS, OP_BN_CONV1X1, OP_QUANT_ROWS, OP_GEMM_I8, OP_NORM_BLOCK) = range(1, 22)
+NORM_NONE, NORM_LAYER, NORM_RMS = 0, 1, 2   # kinds of norm of OP_NORM_BLOCK
 FLAG_HOST_ONLY = 1
 FLAG_EVICT_LRU = 2   # plain LRU instead of the two-class policy (as env EVICT_POLICY=LRU)
 FLAG_NO_PACK = 8   # weights cross the link as they are
@@ -48,6 +49,18 @@ def gemm_noalloc(x, y, c, m, n, k, xs_r, ys_c, ldc, xs_k=1, ys_k=1, nb0=1, nb1=1
     d.nb0, d.nb1, d.xb0, d.xb1, d.yb0, d.yb1, d.cb0, d.cb1 = nb0, nb1, xb0, xb1, yb0, yb1, cb0, cb1
     Server._epilogue(d.ep, **ep)
     return _lib.lib().tp_gemm_noalloc(C.byref(d), C.c_void_p(stream))
+
+
+def _op_arrays(ptrs, ints, floats):
+    return ((C.c_uint64 * max(1, len(ptrs)))(*ptrs), len(ptrs), (C.c_int64 * max(1, len(ints)))(*ints), len(ints),
+            (C.c_float * max(1, len(floats)))(*floats), len(floats))
+
+
+def launch_noalloc(op_id, ptrs, ints=(), floats=(), stream=0):
+    """tp_launch_noalloc: Server.launch on raw device addresses of the current HIP device, enqueued on `stream` (a
+    hipStream_t as an integer, 0 = default stream); OP_QUANT_ROWS, OP_GEMM_I8 and OP_NORM_BLOCK.  Allocates nothing.
+    Returns the status code."""
+    return _lib.lib().tp_launch_noalloc(op_id, *_op_arrays(ptrs, ints, floats), stream)
 
 
 class Server:
@@ -210,10 +223,7 @@ class Server:
                                              layout, int(relu), x_pitch), "tp_bn_inference")
 
     def launch(self, fid, op_id, ptrs, ints=(), floats=()):
-        P = (C.c_uint64 * max(1, len(ptrs)))(*ptrs)
-        I = (C.c_int64 * max(1, len(ints)))(*ints)
-        F = (C.c_float * max(1, len(floats)))(*floats)
-        _chk(self._l.tp_launch(self._h, fid, op_id, P, len(ptrs), I, len(ints), F, len(floats)), "tp_launch")
+        _chk(self._l.tp_launch(self._h, fid, op_id, *_op_arrays(ptrs, ints, floats)), "tp_launch")
 
     def replay(self, fid, input_array, output_array):
         a, p, n = _as_bytes_view(input_array)

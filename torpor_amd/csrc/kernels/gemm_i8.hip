@@ -16,38 +16,99 @@
 
 namespace tpk {
 
+int num_cu();
+
 namespace {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
-typedef int i32x4_any __attribute__((ext_vector_type(4), aligned(1)));
+typedef int i32x4_words __attribute__((ext_vector_type(4), aligned(4)));
 typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 
-// 16 codes at any address.
-__device__ __forceinline__ i32x4 load16(const int8_t* __restrict__ p) { return *reinterpret_cast<const i32x4_any*>(p); }
-
-// The first `left` of 16 codes, 0 behind them; nothing behind them is read.
-__device__ __forceinline__ i32x4 load16(const int8_t* __restrict__ p, int left) {
-    if (left >= 16) return load16(p);
-    i32x4 v = {0, 0, 0, 0};
+// A lane's run of 16 codes in a row that is walked in steps.  128-bit loads need an address that is a multiple of 4 and take more
+// than twice the time at others (8x4096x4096 with a pitch of 4097: 13.9 us, of 4100: 5.9), so rows that do not lie so are read
+// as the five whole words around the run and shifted into place; bytes of the outer two words that belong to a neighbour are
+// read but not used.  ANY = false: every row starts at a multiple of 4.
+template <bool ANY>
+struct Run {
+    const int8_t* p;  // the run's first code, rounded down to a word
+    uint32_t shift;   // bytes between the two
+    __device__ __forceinline__ void set(const int8_t* first) {
+        shift = ANY ? (uint32_t)reinterpret_cast<uintptr_t>(first) & 3 : 0;
+        p = first - shift;
+    }
+    struct Words {
+        i32x4 w;
+        int next;
+    };
+    __device__ __forceinline__ Words load(long at) const {
+        Words v;
+        v.w = *reinterpret_cast<const i32x4_words*>(p + at);
+        // an aligned run has no fifth word: its last one again, so that nothing behind the run is read
+        if constexpr (ANY) v.next = *reinterpret_cast<const int*>(p + at + (shift ? 16 : 12));
+        return v;
+    }
+    __device__ __forceinline__ i32x4 codes(const Words& v) const {
+        if constexpr (!ANY) return v.w;
+        i32x4 r;
 #pragma unroll
-    for (int b = 0; b < 15; ++b)
-        if (b < left) v[b >> 2] |= (int)(uint8_t)p[b] << (8 * (b & 3));
-    return v;
-}
+        for (int k = 0; k < 4; ++k) r[k] = (int)__builtin_amdgcn_alignbyte((uint32_t)(k < 3 ? v.w[k + 1] : v.next), (uint32_t)v.w[k], shift);
+        return r;
+    }
+    // as load, where a row ends inside the run: words that codes() turns into the `left` codes and zeros
+    __device__ __forceinline__ Words load_part(long at, int left) const {
+        if (left >= 16) return load(at);
+        Words v = {i32x4{0, 0, 0, 0}, 0};
+        const int8_t* q = p + at;
+#pragma unroll
+        for (int b = 0; b < (ANY ? 18 : 15); ++b)
+            if (b >= (int)shift && b < left + (int)shift) {
+                const int byte = (int)(uint8_t)q[b] << (8 * (b & 3));
+                if (b < 16) v.w[b >> 2] |= byte;
+                else v.next |= byte;
+            }
+        return v;
+    }
+    // the first `left` of the 16 codes, 0 behind them
+    __device__ __forceinline__ i32x4 part(long at, int left) const { return codes(load_part(at, left)); }
+};
 
-// As apply_act, except that a NaN -- the mark of a row that could not be quantised -- stays one.
+// The epilogue's activations.  A NaN -- the mark of a row that could not be quantised -- stays one under all of them.
+//
+// gelu(v) = v Phi(v) = max(v, 0) - |v| erfc(x) / 2 with x = |v| / sqrt 2, where nothing cancels.  erfc(x) exp(x^2) is a polynomial of degree
+// 8 in t = 1 / (1 + 0.45 x) without constant term, fitted for the least relative error over 0 <= x <= 10 (2.8e-7, so 5e-8 of gelu):
+// twenty instructions where erff takes fifty, which is what a product with gelu and a short inner length is bound by.
+__device__ __forceinline__ float fast_gelu(float v) {
+    const float m = fabsf(v), a = m > 30.f ? 30.f : m;  // not fminf, which would drop a NaN; beyond 30 the second term is 0
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.45f * 0.70710678f, a, 1.f));
+    float p = fmaf(0.06686938554f, t, -0.24030546844f);
+    p = fmaf(p, t, 0.20894774795f);
+    p = fmaf(p, t, 0.04014047235f);
+    p = fmaf(p, t, 0.18876436353f);
+    p = fmaf(p, t, 0.22802931070f);
+    p = fmaf(p, t, 0.25364631414f);
+    p = fmaf(p, t, 0.25390815735f);
+    const float e = __builtin_amdgcn_exp2f(-0.72134752f * a * a);  // exp(-a^2 / 2)
+    return fmaxf(v, 0.f) - 0.5f * a * (p * t) * e;
+}
+__device__ __forceinline__ float fast_sigmoid(float v) {
+    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * v));
+}
 __device__ __forceinline__ float act_keep_nan(float v, int act) {
     if (act == ACT_RELU) return v < 0.f ? 0.f : v;
+    if (act == ACT_GELU) return fast_gelu(v);
+    if (act == ACT_TANH) return tanhf(v);
     if (act == ACT_RELU6) return v < 0.f ? 0.f : v > 6.f ? 6.f : v;
-    return apply_act(v, act);
+    if (act == ACT_SILU) return v * fast_sigmoid(v);
+    if (act == ACT_SIGMOID) return fast_sigmoid(v);
+    return v;
 }
 
 // ------------------------------------------------------------------------------------------------ few outputs
 // Outputs for less than the whole chip as tiles of their own: a workgroup takes 16 FM x 16 FN outputs, its wavefronts split K
 // and add up through LDS.  Every code is used by one wavefront only, so operands go from memory to registers, U groups of 64
 // codes a row at a time.
-template <int FM, int FN, int W, int U>
+template <int FM, int FN, int W, int U, bool ANY>
 __global__ __launch_bounds__(64 * W) void gemm_i8_split_kernel(const GemmI8Args a) {
     constexpr int OUT = 256 * FM * FN;
     __shared__ int sums[W][OUT];
@@ -55,12 +116,12 @@ __global__ __launch_bounds__(64 * W) void gemm_i8_split_kernel(const GemmI8Args 
     const int tiles_n = (a.n + 16 * FN - 1) / (16 * FN);
     const int r0 = (int)(blockIdx.x / tiles_n) * 16 * FM, c0 = (int)(blockIdx.x % tiles_n) * 16 * FN;
     const int row = lane & 15, kl = 16 * (lane >> 4);
-    const int8_t *xp[FM], *wp[FN];
+    Run<ANY> xp[FM], wp[FN];
     // rows past the end read the last one; their results are not stored
 #pragma unroll
-    for (int i = 0; i < FM; ++i) xp[i] = a.x + (long)min(r0 + 16 * i + row, a.m - 1) * a.ldx + kl;
+    for (int i = 0; i < FM; ++i) xp[i].set(a.x + (long)min(r0 + 16 * i + row, a.m - 1) * a.ldx + kl);
 #pragma unroll
-    for (int j = 0; j < FN; ++j) wp[j] = a.w + (long)min(c0 + 16 * j + row, a.n - 1) * a.ldw + kl;
+    for (int j = 0; j < FN; ++j) wp[j].set(a.w + (long)min(c0 + 16 * j + row, a.n - 1) * a.ldw + kl);
 
     i32x4 acc[FM][FN];
 #pragma unroll
@@ -72,28 +133,29 @@ __global__ __launch_bounds__(64 * W) void gemm_i8_split_kernel(const GemmI8Args 
     int g = w * per;
     const int end = min(g + per, groups), fast = min(end, whole);
     for (; g + U <= fast; g += U) {
-        i32x4 xf[FM][U], wf[FN][U];
+        typename Run<ANY>::Words xf[FM][U], wf[FN][U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
 #pragma unroll
-            for (int j = 0; j < FN; ++j) wf[j][u] = load16(wp[j] + ((long)(g + u) << 6));
+            for (int j = 0; j < FN; ++j) wf[j][u] = wp[j].load((long)(g + u) << 6);
 #pragma unroll
-            for (int i = 0; i < FM; ++i) xf[i][u] = load16(xp[i] + ((long)(g + u) << 6));
+            for (int i = 0; i < FM; ++i) xf[i][u] = xp[i].load((long)(g + u) << 6);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int i = 0; i < FM; ++i)
 #pragma unroll
-                for (int j = 0; j < FN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xf[i][u], wf[j][u], acc[i][j], 0, 0, 0);
+                for (int j = 0; j < FN; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xp[i].codes(xf[i][u]), wp[j].codes(wf[j][u]), acc[i][j], 0, 0, 0);
     }
     for (; g < end; ++g) {
         i32x4 xf[FM], wf[FN];
         const int left = a.k - (g << 6) - kl;
 #pragma unroll
-        for (int j = 0; j < FN; ++j) wf[j] = load16(wp[j] + ((long)g << 6), left);
+        for (int j = 0; j < FN; ++j) wf[j] = wp[j].part((long)g << 6, left);
 #pragma unroll
-        for (int i = 0; i < FM; ++i) xf[i] = load16(xp[i] + ((long)g << 6), left);
+        for (int i = 0; i < FM; ++i) xf[i] = xp[i].part((long)g << 6, left);
 #pragma unroll
         for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -130,15 +192,25 @@ struct TileDev {
     int tiles_m, tiles_n;
 };
 
-// BM x BN outputs a workgroup, WGM x WGN wavefronts, K in blocks of 128 codes through LDS.
-template <int BM, int BN, int WGM, int WGN, bool DIRECT>
+// Waits until at most N loads of this wavefront are on their way.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+enum Fetch { DIRECT, WORDS, BYTES };  // chunks of 16 codes straight to LDS; through registers, rows at multiples of 4; at any address
+
+// BM x BN outputs a workgroup, WGM x WGN wavefronts, K in blocks of BK codes through LDS, STAGES of them at a time.
+template <int BM, int BN, int WGM, int WGN, int BK, int STAGES, Fetch HOW>
 __global__ __launch_bounds__(64 * WGM * WGN) void gemm_i8_tile_kernel(const TileDev p) {
-    constexpr int T = 64 * WGM * WGN, NX = BM * 8 / T, NW = BN * 8 / T, NL = NX + NW;
-    constexpr int TM = BM / WGM / 32, TN = BN / WGN / 32, STAGE = (BM + BN) * 128;
-    constexpr int WN = 32 * TN, OP = WN + 8;  // columns of a wavefront, pitch of its output rows in LDS
-    static_assert(BM * 8 % T == 0 && BN * 8 % T == 0 && T / 8 % 16 == 0, "staging in whole rows");
-    static_assert(WGM * WGN * 32 * OP * 4 <= 2 * STAGE, "output rows fit the operands' LDS");
-    __shared__ __attribute__((aligned(128))) int8_t lds[2][STAGE];
+    constexpr bool ANY = HOW == BYTES;
+    constexpr int T = 64 * WGM * WGN, CH = BK / 16, NX = BM * CH / T, NW = BN * CH / T, NL = NX + NW;
+    constexpr int TM = BM / WGM / 16, TN = BN / WGN / 16, STAGE = (BM + BN) * BK, KK = BK / 64;
+    constexpr int WN = 16 * TN, OP = WN + 4;  // columns of a wavefront, pitch of its output rows in LDS
+    constexpr int SPAN = 16 / CH;             // rows that lie side by side in the 64 LDS banks
+    constexpr int OUT = WGM * WGN * 16 * OP * 4, LDS = STAGES * STAGE > OUT ? STAGES * STAGE : OUT;
+    static_assert(BM * CH % T == 0 && BN * CH % T == 0 && T / CH % 16 == 0, "staging in whole rows");
+    __shared__ __attribute__((aligned(256))) int8_t lds[LDS];
     const GemmI8Args& a = p.a;
     const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
 
@@ -155,106 +227,131 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_i8_tile_kernel(const Tile
     const int tm = g * GROUP + in % rows_g, tn = in / rows_g;
     const int r0 = tm * BM, c0 = tn * BN;
 
-    const int K = a.k, steps = (K + 127) >> 7;
-    const int koff = (((t & 7) ^ ((t >> 4) & 7)) << 4);
-    const int8_t* src[NL];
+    const int K = a.k, steps = (K + BK - 1) / BK;
+    const int koff = ((t % CH) ^ ((t / CH / SPAN) % CH)) * 16;
+    Run<ANY> src[NL];
 #pragma unroll
-    for (int j = 0; j < NX; ++j) src[j] = a.x + (long)min(r0 + j * (T / 8) + (t >> 3), a.m - 1) * a.ldx + koff;
+    for (int j = 0; j < NX; ++j) src[j].set(a.x + (long)min(r0 + j * (T / CH) + t / CH, a.m - 1) * a.ldx + koff);
 #pragma unroll
-    for (int j = 0; j < NW; ++j) src[NX + j] = a.w + (long)min(c0 + j * (T / 8) + (t >> 3), a.n - 1) * a.ldw + koff;
+    for (int j = 0; j < NW; ++j) src[NX + j].set(a.w + (long)min(c0 + j * (T / CH) + t / CH, a.n - 1) * a.ldw + koff);
 
-    i32x4 reg[DIRECT ? 1 : NL];
-    auto fetch = [&](int s, int stage) {
-        const int left = K - (s << 7) - koff;  // codes of the row from this lane's chunk on
-        if constexpr (DIRECT) {
+    typename Run<ANY>::Words reg[HOW == DIRECT ? 1 : NL];
+    // loads j0 .. j1-1 of block s, on their way to LDS or to registers
+    auto fetch = [&](int s, int j0, int j1) {
+        const int left = K - s * BK - koff;  // codes of the row from this lane's chunk on
+        if constexpr (HOW == DIRECT) {
+            int8_t* const to = lds + (s % STAGES) * STAGE + w * 1024;
+            if (K - s * BK >= BK) {
 #pragma unroll
-            for (int j = 0; j < NL; ++j) {
-                const int8_t* q = src[j] + ((long)s << 7);
-                if (left <= 0) q = reinterpret_cast<const int8_t*>(&kZeros);
-                __builtin_amdgcn_global_load_lds((gmem_t*)q, (lmem_t*)(&lds[stage][(j * T + w * 64) * 16]), 16, 0, 0);
+                for (int j = j0; j < j1; ++j)
+                    __builtin_amdgcn_global_load_lds((gmem_t*)(src[j].p + (long)s * BK), (lmem_t*)(to + j * T * 16), 16, 0, 0);
+            } else {  // the last block ends inside: chunks behind the end are zeros
+#pragma unroll
+                for (int j = j0; j < j1; ++j) {
+                    const int8_t* q = left > 0 ? src[j].p + (long)s * BK : reinterpret_cast<const int8_t*>(&kZeros);
+                    __builtin_amdgcn_global_load_lds((gmem_t*)q, (lmem_t*)(to + j * T * 16), 16, 0, 0);
+                }
             }
-        } else if (K - (s << 7) >= 128) {
+        } else if (K - s * BK >= BK) {
 #pragma unroll
-            for (int j = 0; j < NL; ++j) reg[j] = load16(src[j] + ((long)s << 7));
+            for (int j = j0; j < j1; ++j) reg[j] = src[j].load((long)s * BK);
         } else {
 #pragma unroll
-            for (int j = 0; j < NL; ++j) reg[j] = load16(src[j] + ((long)s << 7), left);
+            for (int j = j0; j < j1; ++j) reg[j] = src[j].load_part((long)s * BK, left);
         }
     };
-    auto put = [&](int stage) {
-        if constexpr (!DIRECT) {
+    auto put = [&](int s) {
+        if constexpr (HOW != DIRECT) {
 #pragma unroll
-            for (int j = 0; j < NL; ++j) *reinterpret_cast<i32x4*>(&lds[stage][(j * T + t) * 16]) = reg[j];
+            for (int j = 0; j < NL; ++j) *reinterpret_cast<i32x4*>(lds + (s % STAGES) * STAGE + (j * T + t) * 16) = src[j].codes(reg[j]);
         }
     };
 
-    i32x16 acc[TM][TN];
+    i32x4 acc[TM][TN];
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int j = 0; j < TN; ++j)
-#pragma unroll
-            for (int v = 0; v < 16; ++v) acc[i][j][v] = 0;
+        for (int j = 0; j < TN; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
 
     const int wr = (w / WGN) * (BM / WGM), wc = (w % WGN) * (BN / WGN);
-    const int frow = lane & 31, half = lane >> 5, sw = (frow >> 1) & 7;
-    if (steps > 0) {
-        fetch(0, 0);
-        put(0);
-    }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    for (int s = 0; s < steps; ++s) {
-        const int cur = s & 1;
-        if (s + 1 < steps) fetch(s + 1, cur ^ 1);
-        const int8_t* xb = &lds[cur][(wr + frow) * 128];
-        const int8_t* wb = &lds[cur][(BM + wc + frow) * 128];
+    const int frow = lane & 15, part = lane >> 4, sw = (frow / SPAN) % CH;
+    i32x4 xf[2][TM], wf[2][TN];
+    auto frags = [&](int s, int kk, int to) {
+        const int8_t* base = lds + (s % STAGES) * STAGE + frow * BK + (((4 * kk + part) ^ sw) << 4);
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-            const int off = ((2 * kk + half) ^ sw) << 4;
-            i32x4 xf[TM], wf[TN];
+        for (int i = 0; i < TM; ++i) xf[to][i] = *reinterpret_cast<const i32x4*>(base + (wr + i * 16) * BK);
 #pragma unroll
-            for (int i = 0; i < TM; ++i) xf[i] = *reinterpret_cast<const i32x4*>(xb + i * 32 * 128 + off);
+        for (int j = 0; j < TN; ++j) wf[to][j] = *reinterpret_cast<const i32x4*>(base + (BM + wc + j * 16) * BK);
+    };
+    // products q0 .. q1-1 of a group
+    auto multiply = [&](int from, int q0, int q1) {
 #pragma unroll
-            for (int j = 0; j < TN; ++j) wf[j] = *reinterpret_cast<const i32x4*>(wb + j * 32 * 128 + off);
-#pragma unroll
-            for (int i = 0; i < TM; ++i)
-#pragma unroll
-                for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(xf[i], wf[j], acc[i][j], 0, 0, 0);
-        }
-        if (s + 1 < steps) put(cur ^ 1);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-    }
+        for (int q = q0; q < q1; ++q)
+            // w first: a lane's four results are neighbours in a row of y
+            acc[q / TN][q % TN] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[from][q % TN], xf[from][q / TN], acc[q / TN][q % TN], 0, 0, 0);
+    };
 
-    // 32 rows of a wavefront at a time through its share of LDS, so that lanes store four neighbours
-    int* out = reinterpret_cast<int*>(&lds[0][0]) + w * 32 * OP;
-    constexpr int LPR = WN / 4, RPI = 64 / LPR;  // lanes a row, rows an instruction
-    const int oc = 4 * (lane % LPR), col = c0 + wc + oc;
-    float csw[4], cb[4];
+    if (steps > 0) {
+        constexpr int Q = TM * TN;
+        static_assert(KK % 2 == 0 && (HOW == DIRECT || STAGES == 2), "fragment buffers alternate");
+        if constexpr (HOW == DIRECT) {
+            for (int s = 0; s < STAGES; ++s)
+                if (s < steps) fetch(s, 0, NL);
+            if (steps >= STAGES) wait_loads<NL*(STAGES - 1)>();
+            else wait_loads<0>();
+        } else {
+            fetch(0, 0, NL);
+            put(0);
+            if (steps > 1) fetch(1, 0, NL);
+        }
+        __syncthreads();
+        frags(0, 0, 0);
+        for (int s = 0; s < steps; ++s) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const int c = min(col + e, a.n - 1);
-        csw[e] = a.sw[c];
-        cb[e] = a.bias ? a.bias[c] : 0.f;
+            for (int kk = 0; kk < KK; ++kk) {
+                if (kk + 1 < KK) {
+                    frags(s, kk + 1, (kk + 1) & 1);
+                } else if (s + 1 < steps) {
+                    // This wavefront has read all of block s; behind the barrier every wavefront has, and block s + 1 is there.
+                    if constexpr (HOW == DIRECT) {
+                        if (s + STAGES <= steps) wait_loads<NL*(STAGES - 2)>();
+                        else wait_loads<0>();
+                        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the last fragments of block s
+                        __builtin_amdgcn_s_barrier();
+                        asm volatile("" ::: "memory");
+                    } else {
+                        put(s + 1);
+                        __syncthreads();
+                    }
+                    frags(s + 1, 0, 0);
+                }
+                // Loads into the place of a block go out behind the barrier that frees it, one at a time between the products of the
+                // block's last group: a burst of them would hold up every wavefront at once.
+                const int j0 = 0, j1 = kk == KK - 1 ? NL : 0, n = j1 - j0 + 1;
+                const bool more = s + STAGES < steps;
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int j = j0; j < j1; ++j) {
+                    multiply(kk & 1, Q * (j - j0) / n, Q * (j - j0 + 1) / n);
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (more) fetch(s + STAGES, j, j + 1);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                multiply(kk & 1, Q * (n - 1) / n, Q);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
     }
-    const bool whole = col + 4 <= a.n;
+    __syncthreads();
+
+    // four columns of a row
+    auto finish = [&](int row, int col, const i32x4& sum, float s, const float (&csw)[4], const float (&cb)[4], bool plain) {
+        if (row >= a.m || col >= a.n) return;
+        const bool whole = col + 4 <= a.n;
+        f32x4_any v;
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-#pragma unroll
-        for (int j = 0; j < TN; ++j)
-#pragma unroll
-            for (int v = 0; v < 16; ++v) out[(8 * (v >> 2) + 4 * half + (v & 3)) * OP + 32 * j + frow] = acc[i][j][v];
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll 2
-        for (int q = 0; q < 32 / RPI; ++q) {
-            const int rl = q * RPI + lane / LPR, row = r0 + wr + 32 * i + rl;
-            if (row >= a.m || col >= a.n) continue;
-            const i32x4 sum = *reinterpret_cast<const i32x4*>(out + rl * OP + oc);
-            const float s = a.sx[row];
-            f32x4_any v;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = (float)sum[e] * s * csw[e] + cb[e];
+        for (int e = 0; e < 4; ++e) v[e] = (float)sum[e] * s * csw[e] + cb[e];
+        if (!plain) {
             if (a.residual) {
                 const float* rp = a.residual + (long)row * a.ldr + col;
                 if (whole) {
@@ -269,45 +366,110 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_i8_tile_kernel(const Tile
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = act_keep_nan(v[e], a.act);
-            float* yp = a.y + (long)row * a.ldy + col;
-            if (whole) {
-                *reinterpret_cast<f32x4_any*>(yp) = v;
-            } else {
+        }
+        float* yp = a.y + (long)row * a.ldy + col;
+        if (whole) {
+            __builtin_nontemporal_store(v, reinterpret_cast<f32x4_any*>(yp));  // or y drives the operands out of the caches
+        } else {
 #pragma unroll
-                for (int e = 0; e < 3; ++e)
-                    if (col + e < a.n) yp[e] = v[e];
-            }
+            for (int e = 0; e < 3; ++e)
+                if (col + e < a.n) yp[e] = v[e];
+        }
+    };
+    auto column = [&](int col, float (&csw)[4], float (&cb)[4]) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int c = min(col + e, a.n - 1);
+            csw[e] = a.sw[c];
+            cb[e] = a.bias ? a.bias[c] : 0.f;
+        }
+    };
+    // 16 rows of a wavefront at a time through its share of LDS, so that a store covers whole lines of y
+    int* out = reinterpret_cast<int*>(lds) + w * 16 * OP;
+    constexpr int LPR = WN / 4, RPI = 64 / LPR;  // lanes a row, rows an instruction
+    const int oc = 4 * (lane % LPR), col = c0 + wc + oc;
+    float csw[4], cb[4];
+    column(col, csw, cb);
+    const bool plain = !a.residual && a.act == ACT_NONE;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j) *reinterpret_cast<i32x4*>(out + frow * OP + 16 * j + 4 * part) = acc[i][j];
+        __builtin_amdgcn_wave_barrier();
+        const int rl = lane / LPR, row = r0 + wr + 16 * i + rl;
+        if (plain) {
+#pragma unroll
+            for (int q = 0; q < 16; q += RPI)
+                finish(row + q, col, *reinterpret_cast<const i32x4*>(out + (rl + q) * OP + oc), a.sx[min(row + q, a.m - 1)], csw, cb, true);
+        } else {
+#pragma unroll 2
+            for (int q = 0; q < 16; q += RPI)
+                finish(row + q, col, *reinterpret_cast<const i32x4*>(out + (rl + q) * OP + oc), a.sx[min(row + q, a.m - 1)], csw, cb, false);
         }
         __builtin_amdgcn_wave_barrier();
     }
 }
 
-template <int BM, int BN, int WGM, int WGN>
-int launch_tile(const GemmI8Args& a, hipStream_t s, const char* name) {
-    TileDev p;
-    p.a = a;
-    p.tiles_m = (a.m + BM - 1) / BM;
-    p.tiles_n = (a.n + BN - 1) / BN;
-    const long grid = (long)p.tiles_m * p.tiles_n;
-    if (grid * 64 * WGM * WGN > 0xffffffffl) return K_EUNSUPPORTED;
-    const bool direct = ((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.w) | (uintptr_t)a.ldx | (uintptr_t)a.ldw |
-                          (uintptr_t)a.k) & 15) == 0;
-    if (direct)
-        hipLaunchKernelGGL((gemm_i8_tile_kernel<BM, BN, WGM, WGN, true>), dim3((unsigned)grid), dim3(64 * WGM * WGN), 0, s, p);
-    else
-        hipLaunchKernelGGL((gemm_i8_tile_kernel<BM, BN, WGM, WGN, false>), dim3((unsigned)grid), dim3(64 * WGM * WGN), 0, s, p);
-    set_last_kernel(name);
-    return (int)hipGetLastError();
+// How the operands lie: every row at a multiple of 16 and of whole chunks, at a multiple of 4, or anywhere.
+Fetch fetch_of(const GemmI8Args& a) {
+    const uintptr_t rows = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.w) | (uintptr_t)a.ldx | (uintptr_t)a.ldw;
+    return ((rows | (uintptr_t)a.k) & 15) == 0 ? DIRECT : (rows & 3) == 0 ? WORDS : BYTES;
 }
 
+using Launch = void (*)(const GemmI8Args& a, Fetch how, unsigned grid, hipStream_t s);
+
 template <int FM, int FN, int W, int U>
-int launch_split(const GemmI8Args& a, hipStream_t s, const char* name) {
-    const long grid = ((a.m + 16l * FM - 1) / (16 * FM)) * ((a.n + 16l * FN - 1) / (16 * FN));
-    if (grid * 64 * W > 0xffffffffl) return K_EUNSUPPORTED;
-    hipLaunchKernelGGL((gemm_i8_split_kernel<FM, FN, W, U>), dim3((unsigned)grid), dim3(64 * W), 0, s, a);
-    set_last_kernel(name);
-    return (int)hipGetLastError();
+void launch_split(const GemmI8Args& a, Fetch how, unsigned grid, hipStream_t s) {
+    if (how == BYTES) hipLaunchKernelGGL((gemm_i8_split_kernel<FM, FN, W, U, true>), dim3(grid), dim3(64 * W), 0, s, a);
+    else hipLaunchKernelGGL((gemm_i8_split_kernel<FM, FN, W, U, false>), dim3(grid), dim3(64 * W), 0, s, a);
 }
+
+template <int BM, int BN, int WGM, int WGN, int BK, bool REG>
+void launch_tile(const GemmI8Args& a, Fetch how, unsigned grid, hipStream_t s) {
+    const TileDev p = {a, (a.m + BM - 1) / BM, (a.n + BN - 1) / BN};
+    const dim3 g(grid), t(64 * WGM * WGN);
+    if constexpr (REG) {
+        if (how == WORDS) hipLaunchKernelGGL((gemm_i8_tile_kernel<BM, BN, WGM, WGN, BK, 2, WORDS>), g, t, 0, s, p);
+        else hipLaunchKernelGGL((gemm_i8_tile_kernel<BM, BN, WGM, WGN, BK, 2, BYTES>), g, t, 0, s, p);
+    } else {
+        hipLaunchKernelGGL((gemm_i8_tile_kernel<BM, BN, WGM, WGN, BK, 2, DIRECT>), g, t, 0, s, p);
+    }
+}
+
+// What a call takes with one tile or another: 2 + rounds * (first + codes * k / 1024) us, where a round is one tile on each CU, but no
+// less than 2 us and its bytes at 4.5 TB/s.  Of a tile that fills a CU (whole) the last round counts in full, of the others for
+// three tenths, the rest in proportion.  `act` is what a round's activations add (gelu; the large tiles have nothing beside them
+// to hide it).  The numbers are fitted to timings of every tile at 145 shapes (m 1 to 4096, n 256 to 16384, k 256 to 4096); the
+// tile with the least is on average within 2 % of the fastest one, at most 28 %.  Small tiles win as long as there are too few of
+// them to go round; large ones fetch each code less often: at 8192^3 256x256 takes 440 us, 192x128 630, 128x128 620; at
+// 256x1024x4096 32x32 takes 9.9 us, 64x64 13.2, 16x16 16.7.  Rows that are no multiple of 16 go through registers, where more
+// wavefronts pay.
+struct Tile {
+    int m, n, threads;
+    bool whole;
+    float first, codes, act;
+    Launch launch;
+    const char* name;
+};
+const Tile kDirect[] = {
+    {16, 16, 512, true, 0.16f, 0.92f, 0.f, launch_split<1, 1, 8, 4>, "gemm_i8_16x16"},
+    {16, 32, 512, true, 0.38f, 1.36f, 0.f, launch_split<1, 2, 8, 4>, "gemm_i8_16x32"},
+    {32, 32, 1024, true, 0.72f, 1.75f, 0.1f, launch_split<2, 2, 16, 2>, "gemm_i8_32x32"},
+    {32, 64, 512, false, 0.56f, 1.87f, 0.2f, launch_tile<32, 64, 2, 4, 256, false>, "gemm_i8_32x64"},
+    {64, 64, 512, false, 0.87f, 2.45f, 0.4f, launch_tile<64, 64, 4, 2, 256, false>, "gemm_i8_64x64"},
+    {128, 128, 1024, false, 1.79f, 5.23f, 1.8f, launch_tile<128, 128, 4, 4, 128, false>, "gemm_i8_128x128"},
+    {192, 128, 512, false, 3.11f, 6.33f, 5.9f, launch_tile<192, 128, 4, 2, 128, false>, "gemm_i8_192x128"},
+    {256, 256, 512, true, 7.67f, 11.08f, 13.5f, launch_tile<256, 256, 4, 2, 128, false>, "gemm_i8_256x256"},
+};
+const Tile kThroughRegisters[] = {
+    {16, 16, 512, true, 0.95f, 1.18f, 0.f, launch_split<1, 1, 8, 4>, "gemm_i8_16x16"},
+    {16, 32, 512, true, 2.83f, 1.76f, 0.f, launch_split<1, 2, 8, 4>, "gemm_i8_16x32"},
+    {32, 32, 1024, true, 4.26f, 2.20f, 0.1f, launch_split<2, 2, 16, 2>, "gemm_i8_32x32"},
+    {64, 64, 1024, false, 3.67f, 3.44f, 0.4f, launch_tile<64, 64, 4, 4, 256, true>, "gemm_i8_64x64"},
+    {64, 64, 512, false, 2.22f, 4.36f, 0.4f, launch_tile<64, 64, 4, 2, 128, true>, "gemm_i8_64x64"},
+    {128, 128, 1024, false, 4.20f, 7.81f, 1.8f, launch_tile<128, 128, 4, 4, 128, true>, "gemm_i8_128x128"},
+    {192, 128, 512, false, 8.89f, 9.53f, 5.9f, launch_tile<192, 128, 4, 2, 128, true>, "gemm_i8_192x128"},
+};
 
 }  // namespace
 
@@ -316,12 +478,27 @@ int launch_gemm_i8(const GemmI8Args& a, hipStream_t s) {
     if (a.act < ACT_NONE || a.act > ACT_SIGMOID) return K_EINVAL;
     if (a.k > kGemmI8MaxK) return K_EUNSUPPORTED;
     if (a.m == 0 || a.n == 0) return K_OK;
-    const auto tiles = [&](long bm, long bn) { return ((a.m + bm - 1) / bm) * ((a.n + bn - 1) / bn); };
-    if (a.m <= 16) return launch_split<1, 1, 8, 4>(a, s, "gemm_i8_split");
-    if (tiles(64, 64) < 128) return launch_split<2, 2, 8, 4>(a, s, "gemm_i8_split");
-    if (tiles(256, 256) >= 192) return launch_tile<256, 256, 2, 4>(a, s, "gemm_i8_256x256");
-    if (tiles(64, 64) <= 2048) return launch_tile<64, 64, 2, 2>(a, s, "gemm_i8_64x64");
-    return launch_tile<128, 128, 2, 4>(a, s, "gemm_i8_128x128");
+    const Fetch how = fetch_of(a);
+    const Tile *table = how == DIRECT ? kDirect : kThroughRegisters, *best = nullptr;
+    const int count = how == DIRECT ? (int)(sizeof(kDirect) / sizeof(Tile)) : (int)(sizeof(kThroughRegisters) / sizeof(Tile));
+    const float bytes = ((float)a.m + (float)a.n) * (float)a.k + (float)a.m * (float)a.n * (a.residual ? 8.f : 4.f), floor = bytes / 4.5e6f;
+    const bool act = a.act != ACT_NONE && a.act != ACT_RELU && a.act != ACT_RELU6;
+    float least = 0.f;
+    long grid = 0;
+    for (int k = 0; k < count; ++k) {
+        const Tile& t = table[k];
+        const long tiles = (((long)a.m + t.m - 1) / t.m) * (((long)a.n + t.n - 1) / t.n);
+        if (tiles * t.threads > 0xffffffffl) continue;  // the grid's threads have to fit 32 bits
+        const int cus = num_cu();
+        const float full = (float)((tiles + cus - 1) / cus), part = tiles > cus ? (float)tiles / (float)cus : 1.f;
+        const float rounds = t.whole ? full : 0.3f * full + 0.7f * part;
+        const float cost = fmaxf(floor, rounds * (t.first + t.codes * (float)a.k / 1024.f + (act ? t.act : 0.f)));
+        if (!best || cost < least) best = &t, least = cost, grid = tiles;
+    }
+    if (!best) return K_EUNSUPPORTED;
+    best->launch(a, how, (unsigned)grid, s);
+    set_last_kernel(best->name);
+    return (int)hipGetLastError();
 }
 
 }  // namespace tpk

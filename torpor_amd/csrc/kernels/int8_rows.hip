@@ -12,6 +12,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "kernels.hpp"
 
 #pragma clang fp contract(off)  // every fused multiply-add below is written out: one arithmetic in all variants
@@ -24,12 +26,14 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u32_any __attribute__((aligned(1)));
 
-// Elements e .. e+3 of a row, 0 past its end.
-__device__ __forceinline__ f32x4 load4(const float* __restrict__ row, int e, int width) {
+// Group e .. e+3 of a row, 0 past its end.  FOURS: the width is a multiple of 4, so that no group ends inside.  Rows start at an address
+// that is the same for a whole wavefront, so that a lane keeps one 32-bit offset a group for all of a row's tensors.
+template <bool FOURS>
+__device__ __forceinline__ f32x4 load4(const float* __restrict__ row, uint32_t e, uint32_t width) {
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    if (e + 4 <= width) {
+    if (FOURS ? e < width : e + 4 <= width) {
         v = *reinterpret_cast<const f32x4_any*>(row + e);
-    } else if (e < width) {
+    } else if (!FOURS && e < width) {
         v[0] = row[e];
         if (e + 1 < width) v[1] = row[e + 1];
         if (e + 2 < width) v[2] = row[e + 2];
@@ -37,37 +41,91 @@ __device__ __forceinline__ f32x4 load4(const float* __restrict__ row, int e, int
     return v;
 }
 
-__device__ __forceinline__ void store4(float* __restrict__ row, int e, int width, f32x4 v) {
-    if (e + 4 <= width) {
-        *reinterpret_cast<f32x4_any*>(row + e) = v;
-    } else if (e < width) {
+// AROUND: past the caches.  A norm's outputs go so (16384x4096: 237 -> 227 us alone; a layer of 1536 rows 49.5 -> 48.8, others alike);
+// codes that the product reads next do not (the layer 49.5 -> 51.2).
+template <bool FOURS, bool AROUND>
+__device__ __forceinline__ void store4(float* __restrict__ row, uint32_t e, uint32_t width, f32x4 v) {
+    if (FOURS ? e < width : e + 4 <= width) {
+        if (AROUND) __builtin_nontemporal_store(v, reinterpret_cast<f32x4_any*>(row + e));
+        else *reinterpret_cast<f32x4_any*>(row + e) = v;
+    } else if (!FOURS && e < width) {
         row[e] = v[0];
         if (e + 1 < width) row[e + 1] = v[1];
         if (e + 2 < width) row[e + 2] = v[2];
     }
 }
 
-__device__ __forceinline__ void store4(int8_t* __restrict__ row, int e, int width, uint32_t codes) {
-    if (e + 4 <= width) {
-        *reinterpret_cast<u32_any*>(row + e) = codes;
-    } else if (e < width) {
+template <bool FOURS, bool AROUND>
+__device__ __forceinline__ void store4(int8_t* __restrict__ row, uint32_t e, uint32_t width, uint32_t codes) {
+    if (FOURS ? e < width : e + 4 <= width) {
+        if (AROUND) __builtin_nontemporal_store(codes, reinterpret_cast<u32_any*>(row + e));
+        else *reinterpret_cast<u32_any*>(row + e) = codes;
+    } else if (!FOURS && e < width) {
         row[e] = (int8_t)codes;
         if (e + 1 < width) row[e + 1] = (int8_t)(codes >> 8);
         if (e + 2 < width) row[e + 2] = (int8_t)(codes >> 16);
     }
 }
 
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d);
+// Reductions over a wavefront whose result every lane gets: neighbours, pairs, quads and eights by moves within 16 lanes (a mirrored
+// order serves as well as a swap once the lanes on either side agree), then the 16s and the halves by gfx950's row swaps.
+// A tenth of the latency of the same through LDS permutes.
+template <int CTRL>
+__device__ __forceinline__ uint32_t moved(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
+template <int CTRL>
+__device__ __forceinline__ double moved(double v) {
+    return __hiloint2double((int)moved<CTRL>((uint32_t)__double2hiint(v)), (int)moved<CTRL>((uint32_t)__double2loint(v)));
+}
+constexpr int kSwap1 = 0xb1, kSwap2 = 0x4e, kMirror8 = 0x141, kMirror16 = 0x140;
+
+// The two values that a lane's row (16 lanes) and the row beside it hold, and those of the wavefront's halves.
+struct Two {
+    uint32_t a, b;
+};
+__device__ __forceinline__ Two rows16(uint32_t v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return {r[0], r[1]};
+}
+__device__ __forceinline__ Two rows32(uint32_t v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return {r[0], r[1]};
+}
+
+// Sum over groups of N lanes (a power of two).
+template <int N = 64>
+__device__ __forceinline__ double lanes_sum(double v) {
+    if constexpr (N > 1) v += moved<kSwap1>(v);
+    if constexpr (N > 2) v += moved<kSwap2>(v);
+    if constexpr (N > 4) v += moved<kMirror8>(v);
+    if constexpr (N > 8) v += moved<kMirror16>(v);
+    if constexpr (N > 16) {
+        const Two lo = rows16((uint32_t)__double2loint(v)), hi = rows16((uint32_t)__double2hiint(v));
+        v = __hiloint2double((int)hi.a, (int)lo.a) + __hiloint2double((int)hi.b, (int)lo.b);
+    }
+    if constexpr (N > 32) {
+        const Two lo = rows32((uint32_t)__double2loint(v)), hi = rows32((uint32_t)__double2hiint(v));
+        v = __hiloint2double((int)hi.a, (int)lo.a) + __hiloint2double((int)hi.b, (int)lo.b);
+    }
     return v;
 }
 
-__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) {
-        const uint32_t o = (uint32_t)__shfl_xor((int)v, d);
-        v = o > v ? o : v;
+__device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
+
+template <int N = 64>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
+    if constexpr (N > 1) v = umax(v, moved<kSwap1>(v));
+    if constexpr (N > 2) v = umax(v, moved<kSwap2>(v));
+    if constexpr (N > 4) v = umax(v, moved<kMirror8>(v));
+    if constexpr (N > 8) v = umax(v, moved<kMirror16>(v));
+    if constexpr (N > 16) {
+        const Two r = rows16(v);
+        v = umax(r.a, r.b);
+    }
+    if constexpr (N > 32) {
+        const Two r = rows32(v);
+        v = umax(r.a, r.b);
     }
     return v;
 }
@@ -76,14 +134,12 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
 // same and infinities and NaNs come out on top.
 template <int TPR>
 __device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* lds) {
-    v = wave_max(v);
+    v = lanes_max(v);
     if constexpr (TPR > 64) {
-        const int w = threadIdx.x >> 6;
-        if ((threadIdx.x & 63) == 0) lds[w] = v;
+        constexpr int NW = TPR / 64;
+        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
         __syncthreads();
-        v = lds[0];
-#pragma unroll
-        for (int k = 1; k < TPR / 64; ++k) v = lds[k] > v ? lds[k] : v;
+        v = lanes_max<NW>(lds[threadIdx.x % NW]);
     }
     return v;
 }
@@ -126,7 +182,7 @@ __device__ __forceinline__ uint32_t lane_amax(const f32x4 (&v)[ITEMS]) {
 }
 
 // Writes the codes and the scale of a row whose values the lanes hold.
-template <int TPR, int ITEMS>
+template <int TPR, int ITEMS, bool FOURS, bool AROUND>
 __device__ __forceinline__ void quantise_row(const f32x4 (&v)[ITEMS], int lane, int width, int8_t* __restrict__ q,
                                              float* __restrict__ scale, uint32_t* lds) {
     const uint32_t top = row_max<TPR>(lane_amax(v), lds);
@@ -134,22 +190,32 @@ __device__ __forceinline__ void quantise_row(const f32x4 (&v)[ITEMS], int lane, 
     const bool bad = top >= 0x7f800000u;
     const float inv = 1.0f / s;
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i) store4(q, 4 * (lane + TPR * i), width, bad ? 0u : codes_of(v[i], s, inv));
+    for (int i = 0; i < ITEMS; ++i) store4<FOURS, AROUND>(q, 4 * (lane + TPR * i), width, bad ? 0u : codes_of(v[i], s, inv));
     if (lane == 0) *scale = s;
 }
 
-template <int TPR, int ITEMS>
+// The wavefront's place in its workgroup, as a scalar.
+__device__ __forceinline__ int wave() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6); }
+
+template <int TPR, int ITEMS, bool FOURS>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void quant_rows_kernel(const QuantRowsArgs a) {
     constexpr int THREADS = TPR > 256 ? TPR : 256, RPB = THREADS / TPR;
     __shared__ uint32_t lds[2][16];
     const int lane = threadIdx.x % TPR;
-    int turn = 0;
-    for (long row = (long)blockIdx.x * RPB + threadIdx.x / TPR; row < a.rows; row += (long)gridDim.x * RPB, turn ^= 1) {
+    int turn = 0;  // the next row's largest values lie beside this row's, which a slower wavefront may still be reading
+    for (long row = (long)blockIdx.x * RPB + (RPB > 1 ? wave() : 0); row < a.rows; row += (long)gridDim.x * RPB, turn ^= 1) {
         f32x4 v[ITEMS];
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) v[i] = load4(a.x + row * a.ldx, 4 * (lane + TPR * i), a.width);
-        quantise_row<TPR, ITEMS>(v, lane, a.width, a.q + row * a.ldq, a.scale + row, lds[turn]);
+        for (int i = 0; i < ITEMS; ++i) v[i] = load4<FOURS>(a.x + row * a.ldx, 4 * (lane + TPR * i), a.width);
+        quantise_row<TPR, ITEMS, FOURS, false>(v, lane, a.width, a.q + row * a.ldq, a.scale + row, lds[turn]);
     }
+}
+
+// Keeps the compiler from carrying values derived from v (their conversions to double) over this point in registers.
+template <int ITEMS>
+__device__ __forceinline__ void settle(f32x4 (&v)[ITEMS]) {
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) asm volatile("" : "+v"(v[i]));
 }
 
 // Mean and 1 / deviation of a row, in double.  One pass over values that the lanes already hold: sums of v - c and (v - c)^2 with c
@@ -161,8 +227,9 @@ struct Moments {
 
 template <int TPR, int ITEMS>
 __device__ __forceinline__ Moments row_moments(const f32x4 (&v)[ITEMS], int lane, int width, int kind, float eps, double (*lds)[4]) {
-    Moments m;
-    double s1 = 0.0, s2 = 0.0;
+    constexpr int NW = TPR / 64;
+    const int w = threadIdx.x >> 6;
+    double s1 = 0.0, s2 = 0.0, mean = 0.0, var;
     if (kind == 2) {
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i)
@@ -171,124 +238,138 @@ __device__ __forceinline__ Moments row_moments(const f32x4 (&v)[ITEMS], int lane
                 const double d = (double)v[i][k];
                 s2 = fma(d, d, s2);
             }
-        s2 = wave_sum(s2);
-        if constexpr (TPR > 64) {
-            if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6][0] = s2;
+        var = lanes_sum(s2);
+        if constexpr (NW > 1) {
+            if ((threadIdx.x & 63) == 0) lds[w][0] = var;
             __syncthreads();
-            s2 = 0.0;
-#pragma unroll
-            for (int k = 0; k < TPR / 64; ++k) s2 += lds[k][0];
+            var = lanes_sum<NW>(lds[threadIdx.x % NW][0]);
         }
-        m.mean = 0.0;
-        m.rstd = 1.0 / sqrt(s2 / (double)width + (double)eps);
-        return m;
-    }
-    const double c = (double)__shfl(v[0][0], 0);
-    int n = 0;
+    } else {
+        const float first = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v[0][0])));
+        const double c = (double)first;
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i)
+        for (int i = 0; i < ITEMS; ++i) {
+            const int left = width - 4 * (lane + TPR * i);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            if (4 * (lane + TPR * i) + k < width) {
-                const double d = (double)v[i][k] - c;
+            for (int k = 0; k < 4; ++k) {
+                const double d = (double)(k < left ? v[i][k] : first) - c;
                 s1 += d;
                 s2 = fma(d, d, s2);
             }
         }
-    s1 = wave_sum(s1);
-    s2 = wave_sum(s2);
-    double mean, var;
-    if constexpr (TPR > 64) {
-        const int w = threadIdx.x >> 6;
+        s1 = lanes_sum(s1);
+        s2 = lanes_sum(s2);
+        if constexpr (NW > 1) {
+            int n = 0;
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {  // elements of this wavefront's share
-            const int left = width - 4 * (TPR * i + 64 * w);
-            n += left < 0 ? 0 : left > 256 ? 256 : left;
+            for (int i = 0; i < ITEMS; ++i) {  // elements of this wavefront's share
+                const int left = width - 4 * (TPR * i + 64 * w);
+                n += left < 0 ? 0 : left > 256 ? 256 : left;
+            }
+            if ((threadIdx.x & 63) == 0) {
+                lds[w][0] = s1;
+                lds[w][1] = s2;
+                lds[w][2] = c;
+                lds[w][3] = (double)n;
+            }
+            __syncthreads();
+            // a lane for each wavefront's share; the mean is counted from the first one's c
+            const double* share = lds[threadIdx.x % NW];
+            const double from = share[2] - lds[0][2], count = share[3], sum = share[0];
+            const double off = lanes_sum<NW>(fma(count, from, sum)) / (double)width, d = off - from;
+            var = lanes_sum<NW>(fma(d, fma(count, d, -2.0 * sum), share[1]));
+            mean = lds[0][2] + off;
+        } else {
+            const double off = s1 / (double)width;
+            mean = c + off;
+            var = fma(-off, s1, s2);
         }
-        if ((threadIdx.x & 63) == 0) {
-            lds[w][0] = s1;
-            lds[w][1] = s2;
-            lds[w][2] = c;
-            lds[w][3] = (double)n;
-        }
-        __syncthreads();
-        double total = 0.0;
-#pragma unroll
-        for (int k = 0; k < TPR / 64; ++k) total += fma(lds[k][3], lds[k][2] - lds[0][2], lds[k][0]);
-        mean = total / (double)width;  // about the first wavefront's c
-        var = 0.0;
-#pragma unroll
-        for (int k = 0; k < TPR / 64; ++k) {
-            const double d = mean - (lds[k][2] - lds[0][2]);
-            var += fma(d, fma(lds[k][3], d, -2.0 * lds[k][0]), lds[k][1]);
-        }
-        mean += lds[0][2];
-    } else {
-        const double d = s1 / (double)width;
-        mean = c + d;
-        var = fma(-d, s1, s2);
     }
     var = var / (double)width;
     if (var < 0.0) var = 0.0;  // a rounding step below zero; NaN stays NaN
-    m.mean = mean;
-    m.rstd = 1.0 / sqrt(var + (double)eps);
-    return m;
+    return {mean, 1.0 / sqrt(var + (double)eps)};
 }
 
-// t = norm(v) of four elements: (v - mean) * rstd * gamma + beta
-__device__ __forceinline__ double normed(float v, const Moments& m, float gamma, float beta) {
-    return fma(((double)v - m.mean) * m.rstd, (double)gamma, (double)beta);
+// A lane's groups of a vector; a constant where there is none, so that the arithmetic needs no branches.
+template <bool FOURS, int ITEMS>
+__device__ __forceinline__ void load_groups(f32x4 (&v)[ITEMS], const float* __restrict__ row, int first, int step, int width, float absent) {
+    if (row) {
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) v[i] = load4<FOURS>(row, first + step * i, width);
+    } else {
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) v[i] = f32x4{absent, absent, absent, absent};
+    }
 }
 
-template <int TPR, int ITEMS>
-__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_block_kernel(const NormBlockArgs a) {
-    constexpr int THREADS = TPR > 256 ? TPR : 256, RPB = THREADS / TPR;
+template <int TPR, int ITEMS, bool POST, bool PRE, bool FOURS>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? TPR / 256 : 4) void norm_block_kernel(const NormBlockArgs a) {
+    constexpr int THREADS = TPR > 256 ? TPR : 256, RPB = THREADS / TPR, STEP = 4 * TPR;
+    constexpr int PART = ITEMS > 2 ? 2 : ITEMS;  // groups whose gamma, beta and gate are in registers at a time
     __shared__ double sums[2][2][16][4];
     __shared__ uint32_t tops[2][16];
-    const int lane = threadIdx.x % TPR, width = a.width;
-    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+    const int lane = threadIdx.x % TPR, width = a.width, e0 = 4 * lane;
     int turn = 0;  // the next row's sums lie beside this row's, which a slower wavefront may still be reading
-    for (long row = (long)blockIdx.x * RPB + threadIdx.x / TPR; row < a.rows; row += (long)gridDim.x * RPB, turn ^= 1) {
-        f32x4 v[ITEMS];
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i) v[i] = load4(a.x + row * a.ldx, 4 * (lane + TPR * i), width);
+    for (long row = (long)blockIdx.x * RPB + (RPB > 1 ? wave() : 0); row < a.rows; row += (long)gridDim.x * RPB, turn ^= 1) {
+        f32x4 v[ITEMS], rs[ITEMS];
+        load_groups<FOURS>(v, a.x + row * a.ldx, e0, STEP, width, 0.f);
+        load_groups<FOURS>(rs, a.residual ? a.residual + row * a.ldr : nullptr, e0, STEP, width, 0.f);
         Moments post = {0.0, 1.0};
-        if (a.post) post = row_moments<TPR, ITEMS>(v, lane, width, a.post, a.post_eps, sums[turn][0]);
-        const float* gate = nullptr;
-        if (a.gate) gate = a.gate + (a.rows_per_gate ? row / a.rows_per_gate : 0) * (long)width;
+        if constexpr (POST) post = row_moments<TPR, ITEMS>(v, lane, width, a.post, a.post_eps, sums[turn][0]);
+        settle(v);
+        const float* gate = a.gate;
+        if (gate && a.rows_per_gate)
+            gate += (row >> 32 || a.rows_per_gate >> 32 ? row / a.rows_per_gate : (long)((uint32_t)row / (uint32_t)a.rows_per_gate)) * (long)width;
         // the residual stream, rounded to float
         const double b = (double)a.block_scale, c = (double)a.residual_scale;
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            const int e = 4 * (lane + TPR * i);
-            const f32x4 pg = a.post ? load4(a.post_gamma, e, width) : zero, pb = a.post_beta ? load4(a.post_beta, e, width) : zero;
-            const f32x4 gt = gate ? load4(gate, e, width) : zero;
-            const f32x4 rs = a.residual ? load4(a.residual + row * a.ldr, e, width) : zero;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                double t = a.post ? normed(v[i][k], post, pg[k], pb[k]) : (double)v[i][k];
-                if (gate) t *= (double)gt[k];
-                t *= b;
-                if (a.residual) t = fma(c, (double)rs[k], t);
-                v[i][k] = e + k < width ? (float)t : 0.f;
+        for (int j = 0; j < ITEMS; j += PART) {
+            if constexpr (ITEMS > PART) __builtin_amdgcn_sched_barrier(0);  // or all vectors are fetched first, and spill
+            f32x4 pg[PART], pb[PART], gt[PART];
+            if constexpr (POST) {
+                load_groups<FOURS>(pg, a.post_gamma, e0 + j * STEP, STEP, width, 1.f);
+                load_groups<FOURS>(pb, a.post_beta, e0 + j * STEP, STEP, width, 0.f);
             }
-            if (a.h) store4(a.h + row * a.ldh, e, width, v[i]);
+            load_groups<FOURS>(gt, gate, e0 + j * STEP, STEP, width, 1.f);
+#pragma unroll
+            for (int i = 0; i < PART; ++i) {
+                const int e = e0 + (j + i) * STEP;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    double t = (double)v[j + i][k];
+                    if constexpr (POST) t = fma((t - post.mean) * post.rstd, (double)pg[i][k], (double)pb[i][k]);
+                    t *= (double)gt[i][k];
+                    t *= b;
+                    t = fma(c, (double)rs[j + i][k], t);
+                    v[j + i][k] = (float)t;  // 0 past the end, where all factors are
+                }
+                if (a.h) store4<FOURS, true>(a.h + row * a.ldh, e, width, v[j + i]);
+            }
         }
-        if (a.pre) {
+        if constexpr (PRE) {
+            settle(v);
             const Moments pre = row_moments<TPR, ITEMS>(v, lane, width, a.pre, a.pre_eps, sums[turn][1]);
+            settle(v);
 #pragma unroll
-            for (int i = 0; i < ITEMS; ++i) {
-                const int e = 4 * (lane + TPR * i);
-                const f32x4 g = load4(a.pre_gamma, e, width), bt = a.pre_beta ? load4(a.pre_beta, e, width) : zero;
+            for (int j = 0; j < ITEMS; j += PART) {
+                if constexpr (ITEMS > PART) __builtin_amdgcn_sched_barrier(0);
+                f32x4 g[PART], bt[PART];
+                load_groups<FOURS>(g, a.pre_gamma, e0 + j * STEP, STEP, width, 1.f);
+                load_groups<FOURS>(bt, a.pre_beta, e0 + j * STEP, STEP, width, 0.f);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) v[i][k] = e + k < width ? (float)normed(v[i][k], pre, g[k], bt[k]) : 0.f;
+                for (int i = 0; i < PART; ++i) {
+                    const int e = e0 + (j + i) * STEP;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        v[j + i][k] = (float)fma(((double)v[j + i][k] - pre.mean) * pre.rstd, (double)g[i][k], (double)bt[i][k]);
+                    if (a.y) store4<FOURS, true>(a.y + row * a.ldy, e, width, v[j + i]);
+                }
             }
-        }
-        if (a.y) {
+        } else if (a.y) {
 #pragma unroll
-            for (int i = 0; i < ITEMS; ++i) store4(a.y + row * a.ldy, 4 * (lane + TPR * i), width, v[i]);
+            for (int i = 0; i < ITEMS; ++i) store4<FOURS, true>(a.y + row * a.ldy, e0 + i * STEP, width, v[i]);
         }
-        if (a.q) quantise_row<TPR, ITEMS>(v, lane, width, a.q + row * a.ldq, a.scale + row, tops[turn]);
+        if (a.q) quantise_row<TPR, ITEMS, FOURS, true>(v, lane, width, a.q + row * a.ldq, a.scale + row, tops[turn]);
     }
 }
 
@@ -302,16 +383,42 @@ unsigned row_grid(long rows) {
     return (unsigned)(blocks < kMaxGrid ? blocks : kMaxGrid);
 }
 
+template <int TPR, int ITEMS>
+void launch_norm(const NormBlockArgs& a, hipStream_t s) {
+    const dim3 grid(row_grid<TPR>(a.rows)), threads(TPR > 256 ? TPR : 256);
+    const auto go = [&](auto fours) {
+        constexpr bool F = decltype(fours)::value;
+        if (a.post && a.pre) hipLaunchKernelGGL((norm_block_kernel<TPR, ITEMS, true, true, F>), grid, threads, 0, s, a);
+        else if (a.post) hipLaunchKernelGGL((norm_block_kernel<TPR, ITEMS, true, false, F>), grid, threads, 0, s, a);
+        else if (a.pre) hipLaunchKernelGGL((norm_block_kernel<TPR, ITEMS, false, true, F>), grid, threads, 0, s, a);
+        else hipLaunchKernelGGL((norm_block_kernel<TPR, ITEMS, false, false, F>), grid, threads, 0, s, a);
+    };
+    if (a.width % 4 == 0) go(std::true_type{});
+    else go(std::false_type{});
+}
+
+template <int TPR, int ITEMS>
+void launch_quant(const QuantRowsArgs& a, hipStream_t s) {
+    const dim3 grid(row_grid<TPR>(a.rows)), threads(TPR > 256 ? TPR : 256);
+    if (a.width % 4 == 0) hipLaunchKernelGGL((quant_rows_kernel<TPR, ITEMS, true>), grid, threads, 0, s, a);
+    else hipLaunchKernelGGL((quant_rows_kernel<TPR, ITEMS, false>), grid, threads, 0, s, a);
+}
+
 }  // namespace
 
 int launch_quant_rows(const QuantRowsArgs& a, hipStream_t s) {
     if (!a.x || !a.q || !a.scale || a.rows < 0 || a.width < 1) return K_EINVAL;
     if (a.width > kRowOpMaxWidth) return K_EUNSUPPORTED;
     if (a.rows == 0) return K_OK;
-#define QUANT(TPR, ITEMS)                                                                                            \
-    hipLaunchKernelGGL((quant_rows_kernel<TPR, ITEMS>), dim3(row_grid<TPR>(a.rows)), dim3(TPR > 256 ? TPR : 256), 0, s, a)
-    if (a.width <= 1024) QUANT(64, 4);
-    else if (a.width <= 4096) QUANT(256, 4);
+#define QUANT(TPR, ITEMS) launch_quant<TPR, ITEMS>(a, s)
+    // the widest row that each takes; of 257 to 1024 elements a row is a wavefront's where there are enough rows to fill the chip
+    if (a.width <= 256) QUANT(64, 1);
+    else if (a.width <= 512) QUANT(64, 2);
+    else if (a.width <= 1024 && a.rows >= 8192) QUANT(64, 4);
+    else if (a.width <= 1024) QUANT(256, 1);
+    else if (a.width <= 2048) QUANT(256, 2);
+    else if (a.width <= 4096) QUANT(512, 2);
+    else if (a.width <= 8192) QUANT(1024, 2);
     else if (a.width <= 16384) QUANT(1024, 4);
     else QUANT(1024, 16);
 #undef QUANT
@@ -324,10 +431,13 @@ int launch_norm_block(const NormBlockArgs& a, hipStream_t s) {
     if ((a.post && !a.post_gamma) || (a.pre && !a.pre_gamma)) return K_EINVAL;
     if (a.width > kRowOpMaxWidth) return K_EUNSUPPORTED;
     if (a.rows == 0) return K_OK;
-#define NORM(TPR, ITEMS)                                                                                             \
-    hipLaunchKernelGGL((norm_block_kernel<TPR, ITEMS>), dim3(row_grid<TPR>(a.rows)), dim3(TPR > 256 ? TPR : 256), 0, s, a)
-    if (a.width <= 1024) NORM(64, 4);
-    else if (a.width <= 4096) NORM(256, 4);
+#define NORM(TPR, ITEMS) launch_norm<TPR, ITEMS>(a, s)
+    if (a.width <= 256) NORM(64, 1);
+    else if (a.width <= 512) NORM(64, 2);
+    else if (a.width <= 1024) NORM(256, 1);
+    else if (a.width <= 2048) NORM(256, 2);
+    else if (a.width <= 4096) NORM(512, 2);
+    else if (a.width <= 8192) NORM(1024, 2);
     else if (a.width <= 16384) NORM(1024, 4);
     else NORM(1024, 16);
 #undef NORM

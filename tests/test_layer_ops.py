@@ -188,3 +188,39 @@ def test_oracle_gemm_and_norm_against_torch():
     h, _ = ref.norm_block(x, res, gate, 4, post=("rms", g, None, 1e-6), a=0.5, b=2.0)
     rms = torch.nn.functional.rms_norm(torch.from_numpy(x).double(), (20,), torch.from_numpy(g).double(), 1e-6).numpy()
     np.testing.assert_allclose(h, 0.5 * res + 2.0 * gate[[0, 0, 0, 0, 1, 1]] * rms, rtol=1e-12, atol=1e-13)
+
+
+# ------------------------------------------------------------------------------- the served encoder's weights
+def test_quantize_rows_agrees_with_the_operators_definition():
+    from torpor_amd.functions.base import quantize_rows
+
+    rng = np.random.default_rng(1)
+    w = (rng.standard_normal((40, 33)) * np.exp(rng.standard_normal((40, 1)) * 4)).astype(np.float32)
+    w[0] = 0
+    w[1] = np.float32(1e-44)
+    w[2, :] = np.arange(33) - 16.5      # halves of the scale below
+    w[2, 0] = 127
+    for got, want in zip(quantize_rows(w), ref.quant_rows(w)):
+        np.testing.assert_array_equal(got, want)
+    w[3, 5] = np.nan
+    with pytest.raises(ValueError):
+        quantize_rows(w)
+
+
+def test_quantized_bert_uploads_codes_and_scales_for_the_encoder_only():
+    from torpor_amd.functions import bert
+
+    cfg = dict(layers=2, hidden=75, heads=3, ffn=50)
+    weights = bert.init_weights(seed=3, vocab=40, max_pos=16, cfg=cfg)
+    plain = bert.Bert(None, 1, weights=weights, cfg=cfg).weights()
+    mixed = bert.Bert(None, 1, weights=weights, cfg=cfg, quantized=True).weights()
+    matrices = [k for k in plain if k.startswith("encoder.") and plain[k].ndim == 2]
+    assert len(matrices) == 8 and set(mixed) == set(plain) | {k + "_scale" for k in matrices}
+    for k, v in plain.items():
+        if k in matrices:
+            assert mixed[k].dtype == np.int8 and mixed[k].shape == v.shape and mixed[k + "_scale"].shape == v.shape[:1]
+            # half a step of a channel's scale at most (the scale itself is rounded: 1 + 2^-23 covers it)
+            assert (np.abs(mixed[k] * mixed[k + "_scale"][:, None].astype(np.float64) - v) <=
+                    mixed[k + "_scale"][:, None] * 0.5 * (1 + 2.0 ** -16)).all()
+        else:
+            np.testing.assert_array_equal(mixed[k], v)

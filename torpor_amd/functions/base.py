@@ -17,6 +17,17 @@ import numpy as np
 from ..server import ACK_OK, REQ_EXECUTE, REQ_EXECUTE_AFTER_LOAD, REQ_LOAD, REQ_UNLOAD, Server
 
 
+def quantize_rows(w):
+    """Rows of float32 as int8 codes and one float32 scale a row, as OP_QUANT_ROWS makes them: the scale is the largest
+    magnitude over 127 (at least 2^-126), the code the integer nearest to the quotient, halves to even."""
+    w = np.ascontiguousarray(w, dtype=np.float32)
+    if not np.isfinite(w).all():
+        raise ValueError("weights with an infinity or a NaN cannot be quantised")
+    amax = np.abs(w).max(axis=1, initial=0.0).astype(np.float64)
+    scale = np.maximum((amax / 127.0).astype(np.float32), np.float32(2.0 ** -126))
+    return np.rint(w / scale.astype(np.float64)[:, None]).astype(np.int8), scale
+
+
 class Buf:
     """An activation allocation on the server."""
     __slots__ = ("va", "nbytes")

@@ -10,13 +10,19 @@ projection (head width 64; other widths fall back to two head-strided batched GE
 softmax launch), and residual LayerNorm.  Weight names
 and conventions follow `transformers.BertModel` (LayerNorm eps 1e-12, erf GELU, additive mask,
 absolute position + token-type embeddings, tanh pooler on the first token).
+
+`quantized=True`: the encoder's matrices are held as int8 codes with a scale for each output channel -- a quarter of the
+bytes that a swap-in moves -- and multiplied as such: each LayerNorm also writes its rows as codes for the projection that
+reads them, the attention output and the inner activations are quantised by row.  Attention, embeddings, norms, the residual
+stream and the heads stay in float32.
 """
 from collections import OrderedDict
 
 import numpy as np
 
-from ..server import ACT_GELU, ACT_NONE, ACT_TANH, OP_ATTENTION, OP_EMBEDDING, OP_LAYERNORM, OP_SOFTMAX
-from .base import Function
+from ..server import (ACT_GELU, ACT_NONE, ACT_TANH, NORM_LAYER, NORM_NONE, OP_ATTENTION, OP_EMBEDDING, OP_GEMM_I8, OP_LAYERNORM,
+                      OP_NORM_BLOCK, OP_QUANT_ROWS, OP_SOFTMAX)
+from .base import Function, quantize_rows
 
 CONFIGS = {
     "bert-base": dict(layers=12, hidden=768, heads=12, ffn=3072),
@@ -75,8 +81,9 @@ class Bert(Function):
     [B, S] each (transformers.BertForQuestionAnswering)."""
 
     def __init__(self, server, fid, arch="bert-base", batch=1, seq=128, weights=None, seed=0, level=1, cfg=None,
-                 vocab=30522, token_types=False, masked=False):
+                 vocab=30522, token_types=False, masked=False, quantized=False):
         super().__init__(server, fid, level)
+        self.quantized = quantized
         self.token_types, self.masked = token_types, masked
         self.cfg = dict(CONFIGS[arch]) if cfg is None else dict(cfg)
         self.batch, self.seq = batch, seq
@@ -88,7 +95,20 @@ class Bert(Function):
 
     def weights(self):
         """Tensors as uploaded: the Hugging Face state dict, except that each layer's query, key
-        and value matrices (and biases) are stacked into `attention.self.qkv.{weight,bias}`."""
+        and value matrices (and biases) are stacked into `attention.self.qkv.{weight,bias}`.  Quantised: the
+        layers' matrices are int8, each followed by its channels' scales as `weight_scale`."""
+        out = self._float_weights()
+        if not self.quantized:
+            return out
+        mixed = OrderedDict()
+        for k, v in out.items():
+            if k.startswith("encoder.layer.") and k.endswith(".weight") and v.ndim == 2:
+                mixed[k], mixed[k + "_scale"] = quantize_rows(v)
+            else:
+                mixed[k] = v
+        return mixed
+
+    def _float_weights(self):
         out = OrderedDict()
         for k, v in self._weights.items():
             if ".attention.self.key." in k or ".attention.self.value." in k:
@@ -121,6 +141,41 @@ class Bert(Function):
                     xs_r=inp if xs_r is None else xs_r, ys_c=inp, ldc=out, bias=self.w[name + ".bias"], act=act)
         return y
 
+    def _rows_i8(self, tok, width):
+        """Buffers for `tok` quantised rows: (codes, scales)."""
+        return self.alloc(tok * width), self.alloc(tok * 4)
+
+    def _release_i8(self, rows):
+        for b in rows or ():
+            self.release(b)
+
+    def _quantize(self, x, tok, width):
+        q, s = self._rows_i8(tok, width)
+        self.s.launch(self.fid, OP_QUANT_ROWS, [x.va, q.va, s.va], [tok, width])
+        return q, s
+
+    def _project(self, x, tok, inp, out, name, act=ACT_NONE):
+        """act(x . W^T + b) for a matrix of an encoder layer; `x` is a float buffer, or (codes, scales) if quantised."""
+        if not self.quantized:
+            return self._linear(x, tok, inp, out, name, act=act)
+        y = self.alloc(tok * out * 4)
+        self.s.launch(self.fid, OP_GEMM_I8,
+                      [x[0].va, x[1].va, self.w[name + ".weight"], self.w[name + ".weight_scale"], y.va, self.w[name + ".bias"]],
+                      [tok, out, inp, 0, 0, 0, 0, act])
+        return y
+
+    def _norm(self, x, res, tok, name, dst=None, codes=True):
+        """Residual LayerNorm: (float rows, the same as codes and scales for the next projection if quantised)."""
+        if not self.quantized:
+            return self._ln(x, res, tok, name, dst=dst), None
+        H = self.cfg["hidden"]
+        y = self.alloc(tok * H * 4) if dst is None else dst
+        rows = self._rows_i8(tok, H) if codes else None
+        self.s.launch(self.fid, OP_NORM_BLOCK,
+                      [x.va, res.va if res is not None else 0, 0, 0, 0, self.w[name + ".weight"], self.w[name + ".bias"], 0, y.va] +
+                      ([rows[0].va, rows[1].va] if codes else []), [tok, H, NORM_NONE, NORM_LAYER], [1.0, 1.0, 0.0, LN_EPS])
+        return y, rows
+
     def _ln(self, x, res, tok, name, dst=None):
         H = self.cfg["hidden"]
         y = self.alloc(tok * H * 4) if dst is None else dst
@@ -143,13 +198,14 @@ class Bert(Function):
                        self.w["embeddings.position_embeddings.weight"],
                        self.w["embeddings.token_type_embeddings.weight"], emb.va],
                       [tok, S, H, self.vocab, self.type_vocab])
-        h = self._ln(emb, None, tok, "embeddings.LayerNorm")
+        h, hq = self._norm(emb, None, tok, "embeddings.LayerNorm", codes=L > 0)
         self.release(emb)
         scale = 1.0 / float(np.sqrt(dh))
         for i in range(L):
             p = f"encoder.layer.{i}"
             # row t of qkv = [Q | K | V] of token t
-            qkv = self._linear(h, tok, H, 3 * H, p + ".attention.self.qkv")
+            qkv = self._project(hq if self.quantized else h, tok, H, 3 * H, p + ".attention.self.qkv")
+            self._release_i8(hq)
             H3 = 3 * H
             q_va, k_va, v_va = qkv.va, qkv.va + H * 4, qkv.va + 2 * H * 4
             ctx = self.alloc(tok * H * 4)
@@ -170,18 +226,23 @@ class Bert(Function):
                             xb0=A * S * S, xb1=S * S, yb0=S * H3, yb1=dh, cb0=S * H, cb1=dh)
                 self.release(probs)
             self.release(qkv)
-            ao = self._linear(ctx, tok, H, H, p + ".attention.output.dense")
+            cq = self._quantize(ctx, tok, H) if self.quantized else None
+            ao = self._project(cq if self.quantized else ctx, tok, H, H, p + ".attention.output.dense")
+            self._release_i8(cq)
             self.release(ctx)
-            h1 = self._ln(ao, h, tok, p + ".attention.output.LayerNorm")
+            h1, h1q = self._norm(ao, h, tok, p + ".attention.output.LayerNorm")
             self.release(ao)
             self.release(h)
-            inter = self._linear(h1, tok, H, F, p + ".intermediate.dense", act=ACT_GELU)
-            out = self._linear(inter, tok, F, H, p + ".output.dense")
+            inter = self._project(h1q if self.quantized else h1, tok, H, F, p + ".intermediate.dense", act=ACT_GELU)
+            self._release_i8(h1q)
+            iq = self._quantize(inter, tok, F) if self.quantized else None
+            out = self._project(iq if self.quantized else inter, tok, F, H, p + ".output.dense")
+            self._release_i8(iq)
             self.release(inter)
             # One result buffer = [last hidden state | pooled], because the first D2H copy of a request is its
             # completion marker (reference cuda_server.hpp:1044): the last LayerNorm writes straight into it.
             result = self.alloc((tok * H + B * H) * 4) if (i == L - 1 and not self.qa_head) else None
-            h = self._ln(out, h1, tok, p + ".output.LayerNorm", dst=result)
+            h, hq = self._norm(out, h1, tok, p + ".output.LayerNorm", dst=result, codes=i < L - 1)
             self.release(out)
             self.release(h1)
         if self.qa_head:

@@ -584,11 +584,13 @@ def build_function(server, func_id, level, model, batch):
         return efficientnet.EfficientNetB0(server, func_id, batch=batch, seed=func_id, level=level)
     if name == "mobilenet":
         return mobilenet.MobileNetV2(server, func_id, batch=batch, seed=func_id, level=level)
-    if name in ("bert", "bert-base"):
-        return bert.Bert(server, func_id, "bert-base", batch=batch, seq=128, seed=func_id, level=level)
-    if name == "bertqa":
+    int8 = name.endswith("-int8")       # the same models with the encoder's matrices in 8 bits
+    if name in ("bert", "bert-base", "bert-int8"):
+        return bert.Bert(server, func_id, "bert-base", batch=batch, seq=128, seed=func_id, level=level, quantized=int8)
+    if name in ("bertqa", "bertqa-int8"):
         w = bert.init_weights("bert-large", seed=func_id, qa_head=True)
-        return bert.Bert(server, func_id, "bert-large", batch=batch, seq=512, weights=w, level=level, token_types=True)
+        return bert.Bert(server, func_id, "bert-large", batch=batch, seq=512, weights=w, level=level, token_types=True,
+                         quantized=int8)
     raise ValueError(f"unknown model {name}")
 
 

@@ -436,39 +436,40 @@ void launch_tile(const GemmI8Args& a, Fetch how, unsigned grid, hipStream_t s) {
     }
 }
 
-// What a call takes with one tile or another: 2 + rounds * (first + codes * k / 1024) us, where a round is one tile on each CU, but no
-// less than 2 us and its bytes at 4.5 TB/s.  Of a tile that fills a CU (whole) the last round counts in full, of the others for
-// three tenths, the rest in proportion.  `act` is what a round's activations add (gelu; the large tiles have nothing beside them
-// to hide it).  The numbers are fitted to timings of every tile at 145 shapes (m 1 to 4096, n 256 to 16384, k 256 to 4096); the
-// tile with the least is on average within 2 % of the fastest one, at most 28 %.  Small tiles win as long as there are too few of
-// them to go round; large ones fetch each code less often: at 8192^3 256x256 takes 440 us, 192x128 630, 128x128 620; at
-// 256x1024x4096 32x32 takes 9.9 us, 64x64 13.2, 16x16 16.7.  Rows that are no multiple of 16 go through registers, where more
-// wavefronts pay.
+// What a call takes with one tile or another:  2 us + max(bytes / 4.5 TB/s, tile * (1 + more * (rounds - 1)))  with
+//   tile = first + codes * k / 1024 + act us, what one tile takes (act: with gelu, silu, sigmoid or tanh in the epilogue),
+//   rounds = tiles for each CU, rounded up by the share `last`: the rest of a tile that fills a CU takes a round of its own,
+//   more = what a further tile on the CU adds, less than the first where several are on it at once.
+// The numbers are fitted to timings of all tiles at 145 shapes (m 1 to 4096, n 256 to 16384, k 256 to 4096); the tile with the
+// least is on average within 1.6 % of the fastest, at most 21 %.  What they reflect: a CU fetches about 27 bytes a cycle of what lies
+// in L2, so (m + n) * k of a tile counts until its products do; small tiles win as long as there are too few to go round.  At
+// 8192^3 256x256 takes 440 us, 192x128 630; at 1536x4096x1024 with gelu 64x128 takes 15.2, 64x64 20.8, 192x128 19.4; at
+// 256x1024x4096 32x32 takes 9.9 us, 64x64 13.2, 16x16 16.7.  Rows that are no multiple of 16 go through registers.
 struct Tile {
     int m, n, threads;
-    bool whole;
-    float first, codes, act;
+    float first, codes, act, more, last;
     Launch launch;
     const char* name;
 };
 const Tile kDirect[] = {
-    {16, 16, 512, true, 0.16f, 0.92f, 0.f, launch_split<1, 1, 8, 4>, "gemm_i8_16x16"},
-    {16, 32, 512, true, 0.38f, 1.36f, 0.f, launch_split<1, 2, 8, 4>, "gemm_i8_16x32"},
-    {32, 32, 1024, true, 0.72f, 1.75f, 0.1f, launch_split<2, 2, 16, 2>, "gemm_i8_32x32"},
-    {32, 64, 512, false, 0.56f, 1.87f, 0.2f, launch_tile<32, 64, 2, 4, 256, false>, "gemm_i8_32x64"},
-    {64, 64, 512, false, 0.87f, 2.45f, 0.4f, launch_tile<64, 64, 4, 2, 256, false>, "gemm_i8_64x64"},
-    {128, 128, 1024, false, 1.79f, 5.23f, 1.8f, launch_tile<128, 128, 4, 4, 128, false>, "gemm_i8_128x128"},
-    {192, 128, 512, false, 3.11f, 6.33f, 5.9f, launch_tile<192, 128, 4, 2, 128, false>, "gemm_i8_192x128"},
-    {256, 256, 512, true, 7.67f, 11.08f, 13.5f, launch_tile<256, 256, 4, 2, 128, false>, "gemm_i8_256x256"},
+    {16, 16, 512, 0.16f, 0.92f, 0.f, 1.f, 1.f, launch_split<1, 1, 8, 4>, "gemm_i8_16x16"},
+    {16, 32, 512, 0.35f, 1.30f, 0.f, 1.15f, 0.75f, launch_split<1, 2, 8, 4>, "gemm_i8_16x32"},
+    {32, 32, 1024, 0.66f, 1.67f, 0.1f, 1.2f, 1.f, launch_split<2, 2, 16, 2>, "gemm_i8_32x32"},
+    {32, 64, 512, 0.75f, 2.04f, 0.2f, 0.59f, 0.42f, launch_tile<32, 64, 2, 4, 256, false>, "gemm_i8_32x64"},
+    {64, 64, 512, 0.95f, 2.45f, 0.4f, 0.81f, 0.32f, launch_tile<64, 64, 4, 2, 256, false>, "gemm_i8_64x64"},
+    {96, 64, 512, 1.21f, 2.88f, 0.9f, 0.9f, 0.5f, launch_tile<96, 64, 2, 4, 256, false>, "gemm_i8_96x64"},
+    {64, 128, 512, 0.87f, 4.78f, 1.1f, 0.56f, 0.22f, launch_tile<64, 128, 2, 4, 128, false>, "gemm_i8_64x128"},
+    {192, 128, 512, 2.94f, 6.43f, 5.9f, 0.92f, 0.38f, launch_tile<192, 128, 4, 2, 128, false>, "gemm_i8_192x128"},
+    {256, 256, 512, 7.52f, 11.08f, 13.5f, 1.2f, 1.f, launch_tile<256, 256, 4, 2, 128, false>, "gemm_i8_256x256"},
 };
 const Tile kThroughRegisters[] = {
-    {16, 16, 512, true, 0.95f, 1.18f, 0.f, launch_split<1, 1, 8, 4>, "gemm_i8_16x16"},
-    {16, 32, 512, true, 2.83f, 1.76f, 0.f, launch_split<1, 2, 8, 4>, "gemm_i8_16x32"},
-    {32, 32, 1024, true, 4.26f, 2.20f, 0.1f, launch_split<2, 2, 16, 2>, "gemm_i8_32x32"},
-    {64, 64, 1024, false, 3.67f, 3.44f, 0.4f, launch_tile<64, 64, 4, 4, 256, true>, "gemm_i8_64x64"},
-    {64, 64, 512, false, 2.22f, 4.36f, 0.4f, launch_tile<64, 64, 4, 2, 128, true>, "gemm_i8_64x64"},
-    {128, 128, 1024, false, 4.20f, 7.81f, 1.8f, launch_tile<128, 128, 4, 4, 128, true>, "gemm_i8_128x128"},
-    {192, 128, 512, false, 8.89f, 9.53f, 5.9f, launch_tile<192, 128, 4, 2, 128, true>, "gemm_i8_192x128"},
+    {16, 16, 512, 1.23f, 1.38f, 0.f, 0.68f, 0.65f, launch_split<1, 1, 8, 4>, "gemm_i8_16x16"},
+    {16, 32, 512, 2.79f, 1.74f, 0.f, 1.07f, 0.74f, launch_split<1, 2, 8, 4>, "gemm_i8_16x32"},
+    {32, 32, 1024, 4.05f, 2.12f, 0.1f, 1.2f, 1.f, launch_split<2, 2, 16, 2>, "gemm_i8_32x32"},
+    {64, 64, 1024, 3.84f, 3.55f, 0.4f, 0.78f, 0.56f, launch_tile<64, 64, 4, 4, 256, true>, "gemm_i8_64x64"},
+    {64, 64, 512, 2.67f, 4.92f, 0.4f, 0.47f, 0.26f, launch_tile<64, 64, 4, 2, 128, true>, "gemm_i8_64x64"},
+    {128, 128, 1024, 4.06f, 7.63f, 1.8f, 1.2f, 1.f, launch_tile<128, 128, 4, 4, 128, true>, "gemm_i8_128x128"},
+    {192, 128, 512, 8.82f, 9.46f, 5.9f, 1.2f, 0.4f, launch_tile<192, 128, 4, 2, 128, true>, "gemm_i8_192x128"},
 };
 
 }  // namespace
@@ -491,8 +492,9 @@ int launch_gemm_i8(const GemmI8Args& a, hipStream_t s) {
         if (tiles * t.threads > 0xffffffffl) continue;  // the grid's threads have to fit 32 bits
         const int cus = num_cu();
         const float full = (float)((tiles + cus - 1) / cus), part = tiles > cus ? (float)tiles / (float)cus : 1.f;
-        const float rounds = t.whole ? full : 0.3f * full + 0.7f * part;
-        const float cost = fmaxf(floor, rounds * (t.first + t.codes * (float)a.k / 1024.f + (act ? t.act : 0.f)));
+        const float rounds = t.last * full + (1.f - t.last) * part;
+        const float tile = t.first + t.codes * (float)a.k / 1024.f + (act ? t.act : 0.f);
+        const float cost = fmaxf(floor, tile * (1.f + t.more * (rounds - 1.f)));
         if (!best || cost < least) best = &t, least = cost, grid = tiles;
     }
     if (!best) return K_EUNSUPPORTED;

@@ -514,3 +514,31 @@ def test_calls_without_rows_launch_nothing():
     _launch(OP_NORM_BLOCK, [p, 0, 0, 0, 0, p, 0, 0, p + 64], [0, 4, 0, 2], [1.0, 1.0, 0.0, 1e-6])
     torch.cuda.synchronize()
     assert (t == 7).all()
+
+
+@pytest.mark.parametrize("n,k", [(768, 768), (1000, 333), (4096, 1024), (300, 4100)])
+def test_gemm_i8_row_results_do_not_depend_on_the_batch(n, k):
+    """The first row of every batch size, computed by whatever tile the size leads to, has the same bits."""
+    rng = np.random.default_rng(n)
+    xq, sx, wq, sw = _operands(rng, 2100, n, k)
+    bias = rng.standard_normal(n).astype(np.float32)
+    res = rng.standard_normal((2100, n)).astype(np.float32)
+    want = _gemm(xq[:1], sx[:1], wq, sw, bias, res[:1], "gelu")
+    for m in (2, 17, 40, 100, 200, 520, 1100, 2100):
+        got = _gemm(xq[:m], sx[:m], wq, sw, bias, res[:m], "gelu")
+        np.testing.assert_array_equal(got[:1], want, err_msg=str(m))
+
+
+@pytest.mark.parametrize("width", [100, 400, 1000, 1531, 3000, 6000])
+def test_row_operators_do_not_depend_on_the_batch(width):
+    rng = np.random.default_rng(width)
+    big = _Norm(rng, 9000 if width < 2000 else 500, width, "layer", "rms", "one")
+    want = big.run()
+    one = _Norm(rng, 1, width, "layer", "rms", "one")
+    one.x, one.res, one.gate, one.pg, one.pb, one.g, one.be = big.x[7:8], big.res[7:8], big.gate, big.pg, big.pb, big.g, big.be
+    for name, v in one.run().items():
+        np.testing.assert_array_equal(v[0], want[name][7], err_msg=name)
+    q, s = _quant(big.x)
+    q1, s1 = _quant(big.x[7:8])
+    np.testing.assert_array_equal(q1[0], q[7])
+    assert s1[0] == s[7]

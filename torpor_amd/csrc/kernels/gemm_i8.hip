@@ -14,6 +14,8 @@
 #include "kernels.hpp"
 #include "mfma_tile.hpp"
 
+#pragma clang fp contract(off)  // fused multiply-adds are written out: the same bits from every variant
+
 namespace tpk {
 
 int num_cu();
@@ -104,10 +106,16 @@ __device__ __forceinline__ float act_keep_nan(float v, int act) {
     return v;
 }
 
+// An exact sum as a float (one rounding), scaled (two more, the second shared with the bias).
+__device__ __forceinline__ float scaled(int sum, float sx, float sw, float bias) { return fmaf((float)sum * sx, sw, bias); }
+
 // ------------------------------------------------------------------------------------------------ few outputs
-// Outputs for less than the whole chip as tiles of their own: a workgroup takes 16 FM x 16 FN outputs, its wavefronts split K
-// and add up through LDS.  Every code is used by one wavefront only, so operands go from memory to registers, U groups of 64
-// codes a row at a time.
+// Too few outputs to fill the chip with larger tiles, a decoding step above all: a workgroup takes 16 FM x 16 FN outputs, its W
+// wavefronts split K and add up through LDS.  Every code is used by one wavefront only, so operands go from memory to registers, U
+// groups of 64 codes a row at a time.  Bound by the weights' bytes: 8x16384x4096 takes 13.0 us with the operands in the
+// last-level cache, 16.6 us from memory (4.1 TB/s); 1x16384x16384 50 us (5.4 TB/s).  With eight rows or fewer half the matrix
+// unit's work is on repeated rows, which costs nothing next to the loads.  Small calls end at the latency of two trips to memory:
+// 1x768x768 takes 2.6 us back to back, of which 2.2 is what an empty launch takes.
 template <int FM, int FN, int W, int U, bool ANY>
 __global__ __launch_bounds__(64 * W) void gemm_i8_split_kernel(const GemmI8Args a) {
     constexpr int OUT = 256 * FM * FN;
@@ -174,8 +182,7 @@ __global__ __launch_bounds__(64 * W) void gemm_i8_split_kernel(const GemmI8Args 
         int sum = 0;
 #pragma unroll
         for (int k = 0; k < W; ++k) sum += sums[k][o];
-        float v = (float)sum * a.sx[r] * a.sw[c];
-        if (a.bias) v += a.bias[c];
+        float v = scaled(sum, a.sx[r], a.sw[c], a.bias ? a.bias[c] : 0.f);
         if (a.residual) v += a.residual[(long)r * a.ldr + c];
         a.y[(long)r * a.ldy + c] = act_keep_nan(v, a.act);
     }
@@ -192,29 +199,32 @@ struct TileDev {
     int tiles_m, tiles_n;
 };
 
-// Waits until at most N loads of this wavefront are on their way.
-template <int N>
-__device__ __forceinline__ void wait_loads() {
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
-
 enum Fetch { DIRECT, WORDS, BYTES };  // chunks of 16 codes straight to LDS; through registers, rows at multiples of 4; at any address
 
-// BM x BN outputs a workgroup, WGM x WGN wavefronts, K in blocks of BK codes through LDS, STAGES of them at a time.
-template <int BM, int BN, int WGM, int WGN, int BK, int STAGES, Fetch HOW>
+// BM x BN outputs a workgroup, WGM x WGN wavefronts, K in blocks of BK codes through two LDS buffers.
+//
+// A row's 16-code chunks lie in LDS in an order turned by the row (koff / sw below), so that the 16 lanes that read one chunk of 16
+// rows touch all 64 banks; the direct loads, which write LDS in lane order, turn the addresses they read instead.  Fragments of the
+// next 64 codes are read while one group multiplies.  The loads that refill a buffer leave one at a time between the products
+// behind the barrier that frees it: sent off together they held up every wavefront for a thousand cycles of each block
+// (8192^3 with the loads in a burst 572 us, spread 516).  16x16 products rather than 32x32: half the accumulator traffic, which shows
+// because the chip runs at its power limit here (8192^3 of random codes 516 -> 467 us; of zeros, 417 -> 435).  Stores go past the
+// caches, or y drives the operands out of them (467 -> 434 us; 4096^3 74 -> 63).  At 434 us, 2.5 POP/s, the product is as fast as the
+// matrix unit's clock under that limit allows a library's to be (445 us for the same size, without scales).
+template <int BM, int BN, int WGM, int WGN, int BK, Fetch HOW>
 __global__ __launch_bounds__(64 * WGM * WGN) void gemm_i8_tile_kernel(const TileDev p) {
     constexpr bool ANY = HOW == BYTES;
     constexpr int T = 64 * WGM * WGN, CH = BK / 16, NX = BM * CH / T, NW = BN * CH / T, NL = NX + NW;
-    constexpr int TM = BM / WGM / 16, TN = BN / WGN / 16, STAGE = (BM + BN) * BK, KK = BK / 64;
+    constexpr int TM = BM / WGM / 16, TN = BN / WGN / 16, BLOCK = (BM + BN) * BK, KK = BK / 64;
     constexpr int WN = 16 * TN, OP = WN + 4;  // columns of a wavefront, pitch of its output rows in LDS
     constexpr int SPAN = 16 / CH;             // rows that lie side by side in the 64 LDS banks
-    constexpr int OUT = WGM * WGN * 16 * OP * 4, LDS = STAGES * STAGE > OUT ? STAGES * STAGE : OUT;
+    constexpr int OUT = WGM * WGN * 16 * OP * 4, LDS = 2 * BLOCK > OUT ? 2 * BLOCK : OUT;
     static_assert(BM * CH % T == 0 && BN * CH % T == 0 && T / CH % 16 == 0, "staging in whole rows");
     __shared__ __attribute__((aligned(256))) int8_t lds[LDS];
     const GemmI8Args& a = p.a;
     const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
 
-    // workgroup -> tile
+    // workgroup -> tile: each XCD (workgroup id mod 8) takes a run of tiles, eight tile rows deep, whose operands share its L2
     const int total = p.tiles_m * p.tiles_n;
     int id = blockIdx.x;
     {
@@ -240,7 +250,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_i8_tile_kernel(const Tile
     auto fetch = [&](int s, int j0, int j1) {
         const int left = K - s * BK - koff;  // codes of the row from this lane's chunk on
         if constexpr (HOW == DIRECT) {
-            int8_t* const to = lds + (s % STAGES) * STAGE + w * 1024;
+            int8_t* const to = lds + (s & 1) * BLOCK + w * 1024;
             if (K - s * BK >= BK) {
 #pragma unroll
                 for (int j = j0; j < j1; ++j)
@@ -263,7 +273,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_i8_tile_kernel(const Tile
     auto put = [&](int s) {
         if constexpr (HOW != DIRECT) {
 #pragma unroll
-            for (int j = 0; j < NL; ++j) *reinterpret_cast<i32x4*>(lds + (s % STAGES) * STAGE + (j * T + t) * 16) = src[j].codes(reg[j]);
+            for (int j = 0; j < NL; ++j) *reinterpret_cast<i32x4*>(lds + (s & 1) * BLOCK + (j * T + t) * 16) = src[j].codes(reg[j]);
         }
     };
 
@@ -277,7 +287,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_i8_tile_kernel(const Tile
     const int frow = lane & 15, part = lane >> 4, sw = (frow / SPAN) % CH;
     i32x4 xf[2][TM], wf[2][TN];
     auto frags = [&](int s, int kk, int to) {
-        const int8_t* base = lds + (s % STAGES) * STAGE + frow * BK + (((4 * kk + part) ^ sw) << 4);
+        const int8_t* base = lds + (s & 1) * BLOCK + frow * BK + (((4 * kk + part) ^ sw) << 4);
 #pragma unroll
         for (int i = 0; i < TM; ++i) xf[to][i] = *reinterpret_cast<const i32x4*>(base + (wr + i * 16) * BK);
 #pragma unroll
@@ -293,18 +303,23 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_i8_tile_kernel(const Tile
 
     if (steps > 0) {
         constexpr int Q = TM * TN;
-        static_assert(KK % 2 == 0 && (HOW == DIRECT || STAGES == 2), "fragment buffers alternate");
+        static_assert(KK % 2 == 0, "fragment buffers alternate");
         if constexpr (HOW == DIRECT) {
-            for (int s = 0; s < STAGES; ++s)
-                if (s < steps) fetch(s, 0, NL);
-            if (steps >= STAGES) wait_loads<NL*(STAGES - 1)>();
-            else wait_loads<0>();
+            fetch(0, 0, NL);
+            if (steps > 1) {
+                fetch(1, 0, NL);
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");
+            } else {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            }
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
         } else {
             fetch(0, 0, NL);
             put(0);
             if (steps > 1) fetch(1, 0, NL);
+            __syncthreads();
         }
-        __syncthreads();
         frags(0, 0, 0);
         for (int s = 0; s < steps; ++s) {
 #pragma unroll
@@ -314,9 +329,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_i8_tile_kernel(const Tile
                 } else if (s + 1 < steps) {
                     // This wavefront has read all of block s; behind the barrier every wavefront has, and block s + 1 is there.
                     if constexpr (HOW == DIRECT) {
-                        if (s + STAGES <= steps) wait_loads<NL*(STAGES - 2)>();
-                        else wait_loads<0>();
-                        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the last fragments of block s
+                        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
                         __builtin_amdgcn_s_barrier();
                         asm volatile("" ::: "memory");
                     } else {
@@ -325,19 +338,21 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_i8_tile_kernel(const Tile
                     }
                     frags(s + 1, 0, 0);
                 }
-                // Loads into the place of a block go out behind the barrier that frees it, one at a time between the products of the
-                // block's last group: a burst of them would hold up every wavefront at once.
-                const int j0 = 0, j1 = kk == KK - 1 ? NL : 0, n = j1 - j0 + 1;
-                const bool more = s + STAGES < steps;
+                constexpr int n = NL + 1;
+                const bool last = kk == KK - 1;  // the group behind the barrier: loads of block s + 2 between its products
                 __builtin_amdgcn_sched_barrier(0);
+                if (last) {
 #pragma unroll
-                for (int j = j0; j < j1; ++j) {
-                    multiply(kk & 1, Q * (j - j0) / n, Q * (j - j0 + 1) / n);
-                    __builtin_amdgcn_sched_barrier(0);
-                    if (more) fetch(s + STAGES, j, j + 1);
-                    __builtin_amdgcn_sched_barrier(0);
+                    for (int j = 0; j < NL; ++j) {
+                        multiply(kk & 1, Q * j / n, Q * (j + 1) / n);
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (s + 2 < steps) fetch(s + 2, j, j + 1);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    multiply(kk & 1, Q * NL / n, Q);
+                } else {
+                    multiply(kk & 1, 0, Q);
                 }
-                multiply(kk & 1, Q * (n - 1) / n, Q);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
@@ -350,7 +365,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_i8_tile_kernel(const Tile
         const bool whole = col + 4 <= a.n;
         f32x4_any v;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = (float)sum[e] * s * csw[e] + cb[e];
+        for (int e = 0; e < 4; ++e) v[e] = scaled(sum[e], s, csw[e], cb[e]);
         if (!plain) {
             if (a.residual) {
                 const float* rp = a.residual + (long)row * a.ldr + col;
@@ -369,7 +384,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_i8_tile_kernel(const Tile
         }
         float* yp = a.y + (long)row * a.ldy + col;
         if (whole) {
-            __builtin_nontemporal_store(v, reinterpret_cast<f32x4_any*>(yp));  // or y drives the operands out of the caches
+            __builtin_nontemporal_store(v, reinterpret_cast<f32x4_any*>(yp));
         } else {
 #pragma unroll
             for (int e = 0; e < 3; ++e)
@@ -429,10 +444,10 @@ void launch_tile(const GemmI8Args& a, Fetch how, unsigned grid, hipStream_t s) {
     const TileDev p = {a, (a.m + BM - 1) / BM, (a.n + BN - 1) / BN};
     const dim3 g(grid), t(64 * WGM * WGN);
     if constexpr (REG) {
-        if (how == WORDS) hipLaunchKernelGGL((gemm_i8_tile_kernel<BM, BN, WGM, WGN, BK, 2, WORDS>), g, t, 0, s, p);
-        else hipLaunchKernelGGL((gemm_i8_tile_kernel<BM, BN, WGM, WGN, BK, 2, BYTES>), g, t, 0, s, p);
+        if (how == WORDS) hipLaunchKernelGGL((gemm_i8_tile_kernel<BM, BN, WGM, WGN, BK, WORDS>), g, t, 0, s, p);
+        else hipLaunchKernelGGL((gemm_i8_tile_kernel<BM, BN, WGM, WGN, BK, BYTES>), g, t, 0, s, p);
     } else {
-        hipLaunchKernelGGL((gemm_i8_tile_kernel<BM, BN, WGM, WGN, BK, 2, DIRECT>), g, t, 0, s, p);
+        hipLaunchKernelGGL((gemm_i8_tile_kernel<BM, BN, WGM, WGN, BK, DIRECT>), g, t, 0, s, p);
     }
 }
 
@@ -441,7 +456,7 @@ void launch_tile(const GemmI8Args& a, Fetch how, unsigned grid, hipStream_t s) {
 //   rounds = tiles for each CU, rounded up by the share `last`: the rest of a tile that fills a CU takes a round of its own,
 //   more = what a further tile on the CU adds, less than the first where several are on it at once.
 // The numbers are fitted to timings of all tiles at 145 shapes (m 1 to 4096, n 256 to 16384, k 256 to 4096); the tile with the
-// least is on average within 1.6 % of the fastest, at most 21 %.  What they reflect: a CU fetches about 27 bytes a cycle of what lies
+// least is on average within 1.3 % of the fastest, at most 21 %.  What they reflect: a CU fetches about 27 bytes a cycle of what lies
 // in L2, so (m + n) * k of a tile counts until its products do; small tiles win as long as there are too few to go round.  At
 // 8192^3 256x256 takes 440 us, 192x128 630; at 1536x4096x1024 with gelu 64x128 takes 15.2, 64x64 20.8, 192x128 19.4; at
 // 256x1024x4096 32x32 takes 9.9 us, 64x64 13.2, 16x16 16.7.  Rows that are no multiple of 16 go through registers.
@@ -458,7 +473,7 @@ const Tile kDirect[] = {
     {32, 64, 512, 0.75f, 2.04f, 0.2f, 0.59f, 0.42f, launch_tile<32, 64, 2, 4, 256, false>, "gemm_i8_32x64"},
     {64, 64, 512, 0.95f, 2.45f, 0.4f, 0.81f, 0.32f, launch_tile<64, 64, 4, 2, 256, false>, "gemm_i8_64x64"},
     {96, 64, 512, 1.21f, 2.88f, 0.9f, 0.9f, 0.5f, launch_tile<96, 64, 2, 4, 256, false>, "gemm_i8_96x64"},
-    {64, 128, 512, 0.87f, 4.78f, 1.1f, 0.56f, 0.22f, launch_tile<64, 128, 2, 4, 128, false>, "gemm_i8_64x128"},
+    {64, 128, 512, 1.4f, 4.9f, 1.6f, 0.45f, 0.22f, launch_tile<64, 128, 2, 4, 128, false>, "gemm_i8_64x128"},
     {192, 128, 512, 2.94f, 6.43f, 5.9f, 0.92f, 0.38f, launch_tile<192, 128, 4, 2, 128, false>, "gemm_i8_192x128"},
     {256, 256, 512, 7.52f, 11.08f, 13.5f, 1.2f, 1.f, launch_tile<256, 256, 4, 2, 128, false>, "gemm_i8_256x256"},
 };

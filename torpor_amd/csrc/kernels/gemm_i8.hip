@@ -57,19 +57,17 @@ struct Run {
         for (int k = 0; k < 4; ++k) r[k] = (int)__builtin_amdgcn_alignbyte((uint32_t)(k < 3 ? v.w[k + 1] : v.next), (uint32_t)v.w[k], shift);
         return r;
     }
-    // as load, where a row ends inside the run: words that codes() turns into the `left` codes and zeros
+    // as load, where a row ends inside the run: only words that hold some of its `left` codes are read, what is behind them is 0
     __device__ __forceinline__ Words load_part(long at, int left) const {
         if (left >= 16) return load(at);
-        Words v = {i32x4{0, 0, 0, 0}, 0};
-        const int8_t* q = p + at;
-#pragma unroll
-        for (int b = 0; b < (ANY ? 18 : 15); ++b)
-            if (b >= (int)shift && b < left + (int)shift) {
-                const int byte = (int)(uint8_t)q[b] << (8 * (b & 3));
-                if (b < 16) v.w[b >> 2] |= byte;
-                else v.next |= byte;
-            }
-        return v;
+        const int end = left > 0 ? left + (int)shift : 0;  // valid bytes from p + at on
+        auto word = [&](int i) {
+            const int n = end - 4 * i;
+            if (n <= 0) return 0;
+            const int v = *reinterpret_cast<const int*>(p + at + 4 * i);
+            return n >= 4 ? v : v & ((1 << (8 * n)) - 1);
+        };
+        return Words{i32x4{word(0), word(1), word(2), word(3)}, ANY ? word(4) : 0};
     }
     // the first `left` of the 16 codes, 0 behind them
     __device__ __forceinline__ i32x4 part(long at, int left) const { return codes(load_part(at, left)); }
@@ -270,10 +268,33 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_i8_tile_kernel(const Tile
             for (int j = j0; j < j1; ++j) reg[j] = src[j].load_part((long)s * BK, left);
         }
     };
-    auto put = [&](int s) {
+    auto put = [&](int s, int j0, int j1) {
         if constexpr (HOW != DIRECT) {
 #pragma unroll
-            for (int j = 0; j < NL; ++j) *reinterpret_cast<i32x4*>(lds + (s & 1) * BLOCK + (j * T + t) * 16) = src[j].codes(reg[j]);
+            for (int j = j0; j < j1; ++j) *reinterpret_cast<i32x4*>(lds + (s & 1) * BLOCK + (j * T + t) * 16) = src[j].codes(reg[j]);
+        }
+    };
+    // Behind it every wavefront has done with what it read or wrote in LDS so far and, if direct, its loads have arrived.
+    auto meet = [&]() {
+        if constexpr (HOW == DIRECT) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    // Direct loads bring whole chunks; where the last one of x ends inside (K no multiple of 16) what lies behind the end becomes 0,
+    // so that it does not matter what w has there.
+    auto cut = [&](int s) {
+        if constexpr (HOW == DIRECT) {
+            if ((K & 15) == 0 || s != steps - 1) return;
+            const int c = (K - s * BK) >> 4, n = K & 15;
+            for (int r = t; r < BM; r += T) {
+                i32x4* const at = reinterpret_cast<i32x4*>(lds + (s & 1) * BLOCK + r * BK + ((c ^ ((r / SPAN) % CH)) << 4));
+                i32x4 v = *at;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = n >= 4 * i + 4 ? v[i] : n > 4 * i ? v[i] & ((1 << (8 * (n - 4 * i))) - 1) : 0;
+                *at = v;
+            }
+            meet();
         }
     };
 
@@ -304,22 +325,22 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_i8_tile_kernel(const Tile
     if (steps > 0) {
         constexpr int Q = TM * TN;
         static_assert(KK % 2 == 0, "fragment buffers alternate");
+        fetch(0, 0, NL);
         if constexpr (HOW == DIRECT) {
-            fetch(0, 0, NL);
             if (steps > 1) {
                 fetch(1, 0, NL);
                 asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
             } else {
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                meet();
             }
-            __builtin_amdgcn_s_barrier();
-            asm volatile("" ::: "memory");
         } else {
-            fetch(0, 0, NL);
-            put(0);
+            put(0, 0, NL);
             if (steps > 1) fetch(1, 0, NL);
-            __syncthreads();
+            meet();
         }
+        cut(0);
         frags(0, 0, 0);
         for (int s = 0; s < steps; ++s) {
 #pragma unroll
@@ -327,21 +348,17 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_i8_tile_kernel(const Tile
                 if (kk + 1 < KK) {
                     frags(s, kk + 1, (kk + 1) & 1);
                 } else if (s + 1 < steps) {
-                    // This wavefront has read all of block s; behind the barrier every wavefront has, and block s + 1 is there.
-                    if constexpr (HOW == DIRECT) {
-                        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-                        __builtin_amdgcn_s_barrier();
-                        asm volatile("" ::: "memory");
-                    } else {
-                        put(s + 1);
-                        __syncthreads();
-                    }
+                    // this wavefront has read all of block s; behind the barrier every wavefront has, and block s + 1 is there
+                    put(s + 1, 0, NL);
+                    meet();
+                    cut(s + 1);
                     frags(s + 1, 0, 0);
                 }
+                // Loads into the place of a block go out behind the barrier that frees it, one at a time between the products of the
+                // block's last group.
                 constexpr int n = NL + 1;
-                const bool last = kk == KK - 1;  // the group behind the barrier: loads of block s + 2 between its products
                 __builtin_amdgcn_sched_barrier(0);
-                if (last) {
+                if (kk == KK - 1) {
 #pragma unroll
                     for (int j = 0; j < NL; ++j) {
                         multiply(kk & 1, Q * j / n, Q * (j + 1) / n);
@@ -425,10 +442,10 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_i8_tile_kernel(const Tile
     }
 }
 
-// How the operands lie: every row at a multiple of 16 and of whole chunks, at a multiple of 4, or anywhere.
+// How the operands lie: every row at a multiple of 16, at a multiple of 4, or anywhere.
 Fetch fetch_of(const GemmI8Args& a) {
     const uintptr_t rows = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.w) | (uintptr_t)a.ldx | (uintptr_t)a.ldw;
-    return ((rows | (uintptr_t)a.k) & 15) == 0 ? DIRECT : (rows & 3) == 0 ? WORDS : BYTES;
+    return (rows & 15) == 0 ? DIRECT : (rows & 3) == 0 ? WORDS : BYTES;
 }
 
 using Launch = void (*)(const GemmI8Args& a, Fetch how, unsigned grid, hipStream_t s);
@@ -459,7 +476,8 @@ void launch_tile(const GemmI8Args& a, Fetch how, unsigned grid, hipStream_t s) {
 // least is on average within 1.3 % of the fastest, at most 21 %.  What they reflect: a CU fetches about 27 bytes a cycle of what lies
 // in L2, so (m + n) * k of a tile counts until its products do; small tiles win as long as there are too few to go round.  At
 // 8192^3 256x256 takes 440 us, 192x128 630; at 1536x4096x1024 with gelu 64x128 takes 15.2, 64x64 20.8, 192x128 19.4; at
-// 256x1024x4096 32x32 takes 9.9 us, 64x64 13.2, 16x16 16.7.  Rows that are no multiple of 16 go through registers.
+// 256x1024x4096 32x32 takes 9.9 us, 64x64 13.2, 16x16 16.7.  Rows at other addresses than multiples of 16 go through registers
+// (second table, 210 shapes, as near): 3000x4096x4091 with a pitch of 4096 takes 56 us, of 4091 102.
 struct Tile {
     int m, n, threads;
     float first, codes, act, more, last;
@@ -478,13 +496,14 @@ const Tile kDirect[] = {
     {256, 256, 512, 7.52f, 11.08f, 13.5f, 1.2f, 1.f, launch_tile<256, 256, 4, 2, 128, false>, "gemm_i8_256x256"},
 };
 const Tile kThroughRegisters[] = {
-    {16, 16, 512, 1.23f, 1.38f, 0.f, 0.68f, 0.65f, launch_split<1, 1, 8, 4>, "gemm_i8_16x16"},
-    {16, 32, 512, 2.79f, 1.74f, 0.f, 1.07f, 0.74f, launch_split<1, 2, 8, 4>, "gemm_i8_16x32"},
-    {32, 32, 1024, 4.05f, 2.12f, 0.1f, 1.2f, 1.f, launch_split<2, 2, 16, 2>, "gemm_i8_32x32"},
-    {64, 64, 1024, 3.84f, 3.55f, 0.4f, 0.78f, 0.56f, launch_tile<64, 64, 4, 4, 256, true>, "gemm_i8_64x64"},
-    {64, 64, 512, 2.67f, 4.92f, 0.4f, 0.47f, 0.26f, launch_tile<64, 64, 4, 2, 128, true>, "gemm_i8_64x64"},
-    {128, 128, 1024, 4.06f, 7.63f, 1.8f, 1.2f, 1.f, launch_tile<128, 128, 4, 4, 128, true>, "gemm_i8_128x128"},
-    {192, 128, 512, 8.82f, 9.46f, 5.9f, 1.2f, 0.4f, launch_tile<192, 128, 4, 2, 128, true>, "gemm_i8_192x128"},
+    {16, 16, 512, 0.36f, 1.12f, 0.f, 0.95f, 0.83f, launch_split<1, 1, 8, 4>, "gemm_i8_16x16"},
+    {16, 32, 512, 0.70f, 1.72f, 0.f, 0.95f, 0.85f, launch_split<1, 2, 8, 4>, "gemm_i8_16x32"},
+    {32, 32, 1024, 1.56f, 2.03f, 0.1f, 1.2f, 1.f, launch_split<2, 2, 16, 2>, "gemm_i8_32x32"},
+    {64, 64, 1024, 1.97f, 3.82f, 0.4f, 0.75f, 0.66f, launch_tile<64, 64, 4, 4, 256, true>, "gemm_i8_64x64"},
+    {64, 64, 512, 1.15f, 5.44f, 0.4f, 0.49f, 0.23f, launch_tile<64, 64, 4, 2, 128, true>, "gemm_i8_64x64"},
+    {128, 128, 1024, 2.20f, 7.99f, 1.8f, 1.2f, 1.f, launch_tile<128, 128, 4, 4, 128, true>, "gemm_i8_128x128"},
+    {192, 128, 512, 4.90f, 9.50f, 5.9f, 1.2f, 1.f, launch_tile<192, 128, 4, 2, 128, true>, "gemm_i8_192x128"},
+    {256, 128, 1024, 3.65f, 11.08f, 4.f, 1.2f, 1.f, launch_tile<256, 128, 4, 4, 128, true>, "gemm_i8_256x128"},
 };
 
 }  // namespace

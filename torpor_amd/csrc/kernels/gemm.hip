@@ -1131,3 +1131,5 @@ int launch_gemm(const GemmArgs& a, const Workspace& ws, hipStream_t s) {
 }
 
 }  // namespace tpk
+
+#include "gemm_i8.hpp"

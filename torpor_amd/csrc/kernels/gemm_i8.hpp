@@ -1,4 +1,4 @@
-// Matrix product of int8 rows with a scale for each row of x and each row of w, gfx950.
+// Part of gemm.hip: matrix product of int8 rows with a scale for each row of x and each row of w, gfx950.
 //
 //   y[r][c] = act( sx[r] * sw[c] * sum_k x[r][k] * w[c][k] + bias[c] + residual[r][c] )
 //
@@ -7,6 +7,7 @@
 // Operand layout of v_mfma_i32_16x16x64_i8 / v_mfma_i32_32x32x32_i8: a lane holds 16 consecutive k of row (lane % 16 / 32) of
 // each operand, the group of k given by (lane / 16 / 32).  Result register v of a lane: column lane % 16 / 32, row
 // 4 * (lane / 16) + v, or 8 * (v / 4) + 4 * (lane / 32) + v % 4.
+#pragma once
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -20,6 +21,7 @@ namespace tpk {
 
 int num_cu();
 
+namespace i8 {
 namespace {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
@@ -507,8 +509,10 @@ const Tile kThroughRegisters[] = {
 };
 
 }  // namespace
+}  // namespace i8
 
 int launch_gemm_i8(const GemmI8Args& a, hipStream_t s) {
+    using namespace i8;
     if (!a.x || !a.sx || !a.w || !a.sw || !a.y || a.m < 0 || a.n < 0 || a.k < 0) return K_EINVAL;
     if (a.act < ACT_NONE || a.act > ACT_SIGMOID) return K_EINVAL;
     if (a.k > kGemmI8MaxK) return K_EUNSUPPORTED;

@@ -1,4 +1,4 @@
-// Row operators of the 8-bit encoder layer, gfx950: quantisation of rows to int8 codes with a scale, and the norms
+// Part of ops.hip: row operators of the 8-bit encoder layer, gfx950: quantisation of rows to int8 codes with a scale, and the norms
 // around a block with its gate, the residual stream and the quantisation of the result.
 //
 // Both read a row once, keep it in the registers of the lanes that share it and write each output once, so they are bound by
@@ -8,6 +8,7 @@
 //
 // 128-bit accesses of floats need only the floats' own alignment on this hardware, and 32-bit stores of four codes none, so
 // there is one path for every pitch and only a row's last, incomplete group goes element by element.
+#pragma once
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -20,6 +21,7 @@
 
 namespace tpk {
 
+namespace i8 {
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -405,8 +407,10 @@ void launch_quant(const QuantRowsArgs& a, hipStream_t s) {
 }
 
 }  // namespace
+}  // namespace i8
 
 int launch_quant_rows(const QuantRowsArgs& a, hipStream_t s) {
+    using namespace i8;
     if (!a.x || !a.q || !a.scale || a.rows < 0 || a.width < 1) return K_EINVAL;
     if (a.width > kRowOpMaxWidth) return K_EUNSUPPORTED;
     if (a.rows == 0) return K_OK;
@@ -427,6 +431,7 @@ int launch_quant_rows(const QuantRowsArgs& a, hipStream_t s) {
 }
 
 int launch_norm_block(const NormBlockArgs& a, hipStream_t s) {
+    using namespace i8;
     if (!a.x || a.rows < 0 || a.width < 1 || (!a.h && !a.y && !a.q) || (a.q && !a.scale)) return K_EINVAL;
     if ((a.post && !a.post_gamma) || (a.pre && !a.pre_gamma)) return K_EINVAL;
     if (a.width > kRowOpMaxWidth) return K_EUNSUPPORTED;

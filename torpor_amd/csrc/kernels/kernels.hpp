@@ -123,7 +123,7 @@ int launch_softmax(const float* x, const float* mask, float* y, long rows, int w
 int launch_attention(const float* q, const float* k, const float* v, const float* mask, float* out, int B, int A, int S,
                      int dh, long ldq, long ldk, long ldv, long ldo, float scale, hipStream_t s);
 
-// ---- 8-bit encoder layer (int8_rows.hip, gemm_i8.hip).  Pitches in elements, any alignment, no scratch memory. ----
+// ---- 8-bit encoder layer (int8_rows.hpp, gemm_i8.hpp).  Pitches in elements, any alignment, no scratch memory. ----
 constexpr int kRowOpMaxWidth = 65536;  // a row lives in the registers of one workgroup
 constexpr int kGemmI8MaxK = 131071;    // |sum| <= k * 128 * 128 stays below 2^31
 struct QuantRowsArgs {

@@ -946,3 +946,5 @@ int launch_unpack(UnpackArgs& a, hipStream_t s) {
 }
 
 }  // namespace tpk
+
+#include "int8_rows.hpp"

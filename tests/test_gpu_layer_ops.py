@@ -542,3 +542,65 @@ def test_row_operators_do_not_depend_on_the_batch(width):
     q1, s1 = _quant(big.x[7:8])
     np.testing.assert_array_equal(q1[0], q[7])
     assert s1[0] == s[7]
+
+
+# sizes whose costs lead to each of the tiles in turn, K over several blocks with a last one that ends inside a chunk
+TILE_SHAPES = [(5, 300, 1037), (40, 600, 333), (200, 300, 521), (300, 900, 777), (500, 1100, 1037), (1500, 1000, 1100), (1500, 2200, 300),
+               (1900, 2000, 1037), (1500, 4000, 900), (4000, 4100, 700), (96, 760, 1037), (190, 760, 1037), (4090, 4090, 1037)]
+
+
+@pytest.mark.parametrize("pad", ["16", "4", "odd"])
+def test_gemm_i8_every_tile_with_rows_of_every_kind(pad):
+    """Rows at multiples of 16, of 4 and at odd addresses, through every tile that the choice knows for them."""
+    from torpor_amd import _lib
+
+    seen = set()
+    for m, n, k in TILE_SHAPES:
+        rng = np.random.default_rng(m + n)
+        pitch = {"16": (k + 15) // 16 * 16, "4": (k + 3) // 4 * 4 | 4, "odd": k | 1}[pad]
+        ops = _operands(rng, m, n, k)
+        bias = rng.standard_normal(n).astype(np.float32)
+        y = _gemm(*ops, bias, px=pitch, pw=pitch)
+        name = _lib.lib().tp_last_kernel().decode()
+        seen.add(name)
+        # float64 products of float64 numbers below 2^53 are exact here too, and quicker than integer ones
+        p = (ops[0].astype(np.float64) @ ops[2].astype(np.float64).T) * ops[1].astype(np.float64)[:, None] * ops[3].astype(np.float64)
+        assert (np.abs(y - (p + bias)) <= (3 * U * np.abs(p) + U * np.abs(p + bias)) * (1 + 1e-6)).all(), (m, n, k, name)
+    tiles = "16x16 16x32 32x32 64x64 192x128 " + ("32x64 96x64 64x128 256x256" if pad == "16" else "128x128 256x128")
+    assert seen == {"gemm_i8_" + t for t in tiles.split()}
+
+
+def test_more_rows_than_a_grid_has_workgroups():
+    """Rows beyond the largest grid go round the kernels' loop (4 rows a workgroup, 2^20 workgroups)."""
+    rows, width = (1 << 22) + 77, 5
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(rows, width, generator=g, device="cuda")
+    q, s = torch.empty(rows, width, dtype=torch.int8, device="cuda"), torch.empty(rows, device="cuda")
+    _launch(OP_QUANT_ROWS, [x.data_ptr(), q.data_ptr(), s.data_ptr()], [rows, width])
+    y, q2, s2 = torch.empty_like(x), torch.empty_like(q), torch.empty_like(s)
+    gamma = torch.ones(width, device="cuda")
+    _launch(OP_NORM_BLOCK, [x.data_ptr(), 0, 0, 0, 0, gamma.data_ptr(), 0, 0, y.data_ptr(), q2.data_ptr(), s2.data_ptr()],
+            [rows, width, NORM_NONE, NORM_RMS], [1.0, 1.0, 0.0, 1e-6])
+    part = np.r_[0:5, 1000000:1000005, (1 << 22) - 5:(1 << 22) + 77]
+    at = torch.from_numpy(part).cuda()
+    for src, codes, scale in ((x, q, s), (y, q2, s2)):
+        wq, ws = ref.quant_rows(src[at].cpu().numpy())
+        np.testing.assert_array_equal(codes[at].cpu().numpy(), wq)
+        np.testing.assert_array_equal(scale[at].cpu().numpy(), ws)
+    _, want = ref.norm_block(x[at].cpu().numpy(), pre=("rms", np.ones(width), None, float(np.float32(1e-6))))
+    assert (np.abs(y[at].cpu().numpy() - want) <= U * np.abs(want) * 1.001 + 1e-12).all()
+    # every row: codes times scale is within half a step of the value (and a rounding of the scale) everywhere
+    assert bool(((q.float() * s[:, None] - x).abs() <= s[:, None] * 0.5001).all())
+
+
+def test_gemm_i8_very_many_rows():
+    """Nine million rows of five codes: tiles are counted and rows addressed past what 16-row tiles have in a grid's 2^32 threads."""
+    m, n, k = 9_000_001, 3, 5
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x = torch.randint(-127, 128, (m, k), generator=g, device="cuda", dtype=torch.int8)
+    w = torch.randint(-127, 128, (n, k), generator=g, device="cuda", dtype=torch.int8)
+    sx, sw = torch.rand(m, generator=g, device="cuda"), torch.ones(n, device="cuda")
+    y = torch.empty(m, n, device="cuda")
+    _launch(OP_GEMM_I8, [x.data_ptr(), sx.data_ptr(), w.data_ptr(), sw.data_ptr(), y.data_ptr()], [m, n, k])
+    want = (x.float() @ w.float().t()) * sx[:, None]      # sums below 2^24: exact; one rounding on either side
+    assert bool((y == want).all())

@@ -9,8 +9,10 @@ from oracle import models as om
 from oracle import ops as ref
 from tests.test_gpu_layer_ops import U, _gemm_error
 from tests.test_gpu_models import _check_swap_identity, _cycle
+from tests.test_gpu_wire import gpu_wire_server  # noqa: F401  (a server process, as a fixture)
+from torpor_amd import client as wire
 from torpor_amd.functions import bert
-from torpor_amd.server import ACT_GELU, OP_GEMM_I8, OP_NORM_BLOCK, OP_QUANT_ROWS
+from torpor_amd.server import ACT_GELU, OP_GEMM_I8, OP_NORM_BLOCK, OP_QUANT_ROWS, Server
 
 pytestmark = pytest.mark.gpu
 
@@ -124,3 +126,44 @@ def test_quantized_bert_base_moves_fewer_bytes(gpu_server):
         fn.unload()
     elements = 12 * (4 * 768 * 768 + 2 * 768 * 3072)
     assert sizes[False] - sizes[True] == 3 * elements - 12 * 4 * (3 * 768 + 768 + 3072 + 768)
+
+
+def _small():
+    cfg = dict(layers=2, hidden=128, heads=2, ffn=200)
+    weights = bert.init_weights(seed=2, vocab=500, max_pos=64, cfg=cfg)
+    ids = torch.randint(0, 500, (2, 48), generator=torch.Generator().manual_seed(1)).numpy()
+    return cfg, weights, ids
+
+
+def test_quantized_bert_over_the_wire(gpu_wire_server):  # noqa: F811
+    """int8 weights and the three operators through the message protocol: the same bits as in process, warm, cold and replayed."""
+    cfg, weights, ids = _small()
+    with Server(mem_limit_bytes=1 << 30, pool_bytes=2 << 30) as local:
+        want = bert.Bert(local, 0, batch=2, seq=48, weights=weights, cfg=cfg, quantized=True).register([ids])
+    with wire.RemoteServer(gpu_wire_server, client_id=21) as rs:
+        fn = bert.Bert(rs, 21, batch=2, seq=48, weights=weights, cfg=cfg, quantized=True)
+        got = [fn.register([ids]), fn.invoke([ids], replay=False)]
+        fn.unload()
+        got.append(fn.invoke([ids]))
+        fn.unload()
+    for answer in got:
+        for a, b in zip(answer, want):
+            np.testing.assert_array_equal(a, b)
+
+
+def test_quantized_bert_as_a_captured_graph(monkeypatch):
+    """Warm requests launch the operators as one graph; other inputs between them, every answer that of the op-by-op path."""
+    monkeypatch.setenv("TORPOR_GRAPH_MIN_OPS", "4")
+    cfg, weights, ids = _small()
+    other = np.ascontiguousarray(ids[:, ::-1])
+    with Server(mem_limit_bytes=1 << 30, pool_bytes=2 << 30) as s:
+        fn = bert.Bert(s, 3, batch=2, seq=48, weights=weights, cfg=cfg, quantized=True)
+        first = fn.register([ids])
+        second = [a.copy() for a in fn.invoke([other], replay=False)]
+        for turn in range(6):
+            for x, want in ((ids, first), (other, second)):
+                for a, b in zip(fn.invoke([x]), want):
+                    np.testing.assert_array_equal(a, b, err_msg=str(turn))
+        fn.unload()
+        for a, b in zip(fn.invoke([ids]), first):
+            np.testing.assert_array_equal(a, b)

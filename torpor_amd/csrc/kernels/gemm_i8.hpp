@@ -12,6 +12,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "kernels.hpp"
 #include "mfma_tile.hpp"
 
@@ -104,6 +106,12 @@ __device__ __forceinline__ float act_keep_nan(float v, int act) {
     if (act == ACT_SILU) return v * fast_sigmoid(v);
     if (act == ACT_SIGMOID) return fast_sigmoid(v);
     return v;
+}
+
+template <int ACT>
+__device__ __forceinline__ void act4(f32x4_any& v) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = act_keep_nan(v[e], ACT);
 }
 
 // An exact sum as a float (one rounding), scaled (two more, the second shared with the bias).
@@ -200,6 +208,8 @@ struct TileDev {
 };
 
 enum Fetch { DIRECT, WORDS, BYTES };  // chunks of 16 codes straight to LDS; through registers, rows at multiples of 4; at any address
+
+enum Rest { NOTHING, GELU, ANYTHING };  // what an epilogue does beyond scaling
 
 // BM x BN outputs a workgroup, WGM x WGN wavefronts, K in blocks of BK codes through two LDS buffers.
 //
@@ -379,13 +389,14 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_i8_tile_kernel(const Tile
     __syncthreads();
 
     // four columns of a row
-    auto finish = [&](int row, int col, const i32x4& sum, float s, const float (&csw)[4], const float (&cb)[4], bool plain) {
+    auto finish = [&](int row, int col, const i32x4& sum, float s, const float (&csw)[4], const float (&cb)[4], auto what) {
+        constexpr Rest rest = decltype(what)::value;
         if (row >= a.m || col >= a.n) return;
         const bool whole = col + 4 <= a.n;
         f32x4_any v;
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = scaled(sum[e], s, csw[e], cb[e]);
-        if (!plain) {
+        if constexpr (rest != NOTHING) {
             if (a.residual) {
                 const float* rp = a.residual + (long)row * a.ldr + col;
                 if (whole) {
@@ -398,8 +409,12 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_i8_tile_kernel(const Tile
                         if (col + e < a.n) v[e] += rp[e];
                 }
             }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = act_keep_nan(v[e], a.act);
+            if constexpr (rest == GELU) act4<ACT_GELU>(v);
+            else if (a.act == ACT_RELU) act4<ACT_RELU>(v);
+            else if (a.act == ACT_TANH) act4<ACT_TANH>(v);
+            else if (a.act == ACT_RELU6) act4<ACT_RELU6>(v);
+            else if (a.act == ACT_SILU) act4<ACT_SILU>(v);
+            else if (a.act == ACT_SIGMOID) act4<ACT_SIGMOID>(v);
         }
         float* yp = a.y + (long)row * a.ldy + col;
         if (whole) {
@@ -424,22 +439,20 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_i8_tile_kernel(const Tile
     const int oc = 4 * (lane % LPR), col = c0 + wc + oc;
     float csw[4], cb[4];
     column(col, csw, cb);
-    const bool plain = !a.residual && a.act == ACT_NONE;
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
 #pragma unroll
         for (int j = 0; j < TN; ++j) *reinterpret_cast<i32x4*>(out + frow * OP + 16 * j + 4 * part) = acc[i][j];
         __builtin_amdgcn_wave_barrier();
         const int rl = lane / LPR, row = r0 + wr + 16 * i + rl;
-        if (plain) {
+        const auto rows = [&](auto what) {
 #pragma unroll
             for (int q = 0; q < 16; q += RPI)
-                finish(row + q, col, *reinterpret_cast<const i32x4*>(out + (rl + q) * OP + oc), a.sx[min(row + q, a.m - 1)], csw, cb, true);
-        } else {
-#pragma unroll 2
-            for (int q = 0; q < 16; q += RPI)
-                finish(row + q, col, *reinterpret_cast<const i32x4*>(out + (rl + q) * OP + oc), a.sx[min(row + q, a.m - 1)], csw, cb, false);
-        }
+                finish(row + q, col, *reinterpret_cast<const i32x4*>(out + (rl + q) * OP + oc), a.sx[min(row + q, a.m - 1)], csw, cb, what);
+        };
+        if (a.act == ACT_GELU) rows(std::integral_constant<Rest, GELU>{});
+        else if (a.residual || a.act != ACT_NONE) rows(std::integral_constant<Rest, ANYTHING>{});
+        else rows(std::integral_constant<Rest, NOTHING>{});
         __builtin_amdgcn_wave_barrier();
     }
 }
@@ -470,42 +483,47 @@ void launch_tile(const GemmI8Args& a, Fetch how, unsigned grid, hipStream_t s) {
     }
 }
 
-// What a call takes with one tile or another:  2 us + max(bytes / 4.5 TB/s, tile * (1 + more * (rounds - 1)))  with
+// What a call takes with one tile or another:  2 us + sqrt((bytes / 5.6 TB/s)^2 + work^2), so the tile with the least work is taken:
+//   work = tile * (1 + more * (rounds - 1)),  next for more from a CU's tile number `held` + 1 on,
 //   tile = first + codes * k / 1024 + act us, what one tile takes (act: with gelu, silu, sigmoid or tanh in the epilogue),
-//   rounds = tiles for each CU, rounded up by the share `last`: the rest of a tile that fills a CU takes a round of its own,
-//   more = what a further tile on the CU adds, less than the first where several are on it at once.
-// The numbers are fitted to timings of all tiles at 145 shapes (m 1 to 4096, n 256 to 16384, k 256 to 4096); the tile with the
-// least is on average within 1.3 % of the fastest, at most 21 %.  What they reflect: a CU fetches about 27 bytes a cycle of what lies
-// in L2, so (m + n) * k of a tile counts until its products do; small tiles win as long as there are too few to go round.  At
-// 8192^3 256x256 takes 440 us, 192x128 630; at 1536x4096x1024 with gelu 64x128 takes 15.2, 64x64 20.8, 192x128 19.4; at
-// 256x1024x4096 32x32 takes 9.9 us, 64x64 13.2, 16x16 16.7.  Rows at other addresses than multiples of 16 go through registers
-// (second table, 210 shapes, as near): 3000x4096x4091 with a pitch of 4096 takes 56 us, of 4091 102.
+//   rounds = tiles for each CU, rounded up by the share `last`,
+//   held = tiles that a CU's LDS and wavefronts hold at once (second table: not told apart), more = what one beside others adds.
+// The numbers are fitted to timings of all tiles at 870 shapes, most of them random (m 1 to 16384, n 128 to 32768, k 64 to 16384, with
+// gelu and without): the tile taken is on average within 1 % of the fastest, at most 26 %, and within 1.1 % at 120 random shapes that
+// the fit has not seen.  What they reflect: a CU fetches about 27 bytes a cycle of what lies in L2, so (m + n) * k of a tile counts until
+// its products do; small tiles win as long as there are too few to go round; 256x256 is alone on its CU, so its epilogue has nothing to
+// hide behind and it needs a long k.  At 8192^3 256x256 takes 440 us, 192x128 630; at 8192x8192x1024 with gelu 192x128 takes 116, 256x256
+// 127, 64x128 134; at 1536x4096x1024 with gelu 64x128 takes 14.9, 192x128 16.1, 64x64 20.9; at 256x1024x4096 32x32 takes 9.9 us, 64x64
+// 13.2, 16x16 16.7.  Rows at other addresses than multiples of 16 go through registers (second table, 260 shapes, within 0.9 %, at most
+// 20 %): 3000x4096x4091 with a pitch of 4096 takes 56 us, of 4091 102.
 struct Tile {
     int m, n, threads;
-    float first, codes, act, more, last;
+    float first, codes, act, more;
+    int held;
+    float next, last;
     Launch launch;
     const char* name;
 };
 const Tile kDirect[] = {
-    {16, 16, 512, 0.16f, 0.92f, 0.f, 1.f, 1.f, launch_split<1, 1, 8, 4>, "gemm_i8_16x16"},
-    {16, 32, 512, 0.35f, 1.30f, 0.f, 1.15f, 0.75f, launch_split<1, 2, 8, 4>, "gemm_i8_16x32"},
-    {32, 32, 1024, 0.66f, 1.67f, 0.1f, 1.2f, 1.f, launch_split<2, 2, 16, 2>, "gemm_i8_32x32"},
-    {32, 64, 512, 0.75f, 2.04f, 0.2f, 0.59f, 0.42f, launch_tile<32, 64, 2, 4, 256, false>, "gemm_i8_32x64"},
-    {64, 64, 512, 0.95f, 2.45f, 0.4f, 0.81f, 0.32f, launch_tile<64, 64, 4, 2, 256, false>, "gemm_i8_64x64"},
-    {96, 64, 512, 1.21f, 2.88f, 0.9f, 0.9f, 0.5f, launch_tile<96, 64, 2, 4, 256, false>, "gemm_i8_96x64"},
-    {64, 128, 512, 1.4f, 4.9f, 1.6f, 0.45f, 0.22f, launch_tile<64, 128, 2, 4, 128, false>, "gemm_i8_64x128"},
-    {192, 128, 512, 2.94f, 6.43f, 5.9f, 0.92f, 0.38f, launch_tile<192, 128, 4, 2, 128, false>, "gemm_i8_192x128"},
-    {256, 256, 512, 7.52f, 11.08f, 13.5f, 1.2f, 1.f, launch_tile<256, 256, 4, 2, 128, false>, "gemm_i8_256x256"},
+    {16, 16, 512, 0.26f, 0.67f, 0.01f, 0.96f, 4, 1.25f, 0.81f, launch_split<1, 1, 8, 4>, "gemm_i8_16x16"},
+    {16, 32, 512, 0.55f, 1.06f, 0.05f, 0.98f, 4, 0.99f, 1.f, launch_split<1, 2, 8, 4>, "gemm_i8_16x32"},
+    {32, 32, 1024, 0.87f, 1.38f, 0.f, 1.54f, 2, 1.39f, 0.91f, launch_split<2, 2, 16, 2>, "gemm_i8_32x32"},
+    {32, 64, 512, 1.11f, 2.13f, 0.24f, 0.36f, 3, 0.57f, 1.f, launch_tile<32, 64, 2, 4, 256, false>, "gemm_i8_32x64"},
+    {64, 64, 512, 1.47f, 2.58f, 0.23f, 0.37f, 2, 0.87f, 0.93f, launch_tile<64, 64, 4, 2, 256, false>, "gemm_i8_64x64"},
+    {96, 64, 512, 1.89f, 2.72f, 0.43f, 0.64f, 2, 0.8f, 0.58f, launch_tile<96, 64, 2, 4, 256, false>, "gemm_i8_96x64"},
+    {64, 128, 512, 1.49f, 4.45f, 0.68f, 0.38f, 3, 0.83f, 1.f, launch_tile<64, 128, 2, 4, 128, false>, "gemm_i8_64x128"},
+    {192, 128, 512, 2.74f, 6.62f, 2.44f, 0.98f, 2, 0.86f, 0.43f, launch_tile<192, 128, 4, 2, 128, false>, "gemm_i8_192x128"},
+    {256, 256, 512, 8.66f, 12.55f, 5.71f, 0.f, 1, 1.13f, 0.97f, launch_tile<256, 256, 4, 2, 128, false>, "gemm_i8_256x256"},
 };
 const Tile kThroughRegisters[] = {
-    {16, 16, 512, 0.36f, 1.12f, 0.f, 0.95f, 0.83f, launch_split<1, 1, 8, 4>, "gemm_i8_16x16"},
-    {16, 32, 512, 0.70f, 1.72f, 0.f, 0.95f, 0.85f, launch_split<1, 2, 8, 4>, "gemm_i8_16x32"},
-    {32, 32, 1024, 1.56f, 2.03f, 0.1f, 1.2f, 1.f, launch_split<2, 2, 16, 2>, "gemm_i8_32x32"},
-    {64, 64, 1024, 1.97f, 3.82f, 0.4f, 0.75f, 0.66f, launch_tile<64, 64, 4, 4, 256, true>, "gemm_i8_64x64"},
-    {64, 64, 512, 1.15f, 5.44f, 0.4f, 0.49f, 0.23f, launch_tile<64, 64, 4, 2, 128, true>, "gemm_i8_64x64"},
-    {128, 128, 1024, 2.20f, 7.99f, 1.8f, 1.2f, 1.f, launch_tile<128, 128, 4, 4, 128, true>, "gemm_i8_128x128"},
-    {192, 128, 512, 4.90f, 9.50f, 5.9f, 1.2f, 1.f, launch_tile<192, 128, 4, 2, 128, true>, "gemm_i8_192x128"},
-    {256, 128, 1024, 3.65f, 11.08f, 4.f, 1.2f, 1.f, launch_tile<256, 128, 4, 4, 128, true>, "gemm_i8_256x128"},
+    {16, 16, 512, 0.36f, 1.12f, 0.f, 0.95f, 1, 0.95f, 0.83f, launch_split<1, 1, 8, 4>, "gemm_i8_16x16"},
+    {16, 32, 512, 0.7f, 1.72f, 0.f, 0.95f, 1, 0.95f, 0.85f, launch_split<1, 2, 8, 4>, "gemm_i8_16x32"},
+    {32, 32, 1024, 1.56f, 2.03f, 0.1f, 1.2f, 1, 1.2f, 1.f, launch_split<2, 2, 16, 2>, "gemm_i8_32x32"},
+    {64, 64, 1024, 1.97f, 3.82f, 0.4f, 0.75f, 1, 0.75f, 0.66f, launch_tile<64, 64, 4, 4, 256, true>, "gemm_i8_64x64"},
+    {64, 64, 512, 1.15f, 5.44f, 0.4f, 0.49f, 1, 0.49f, 0.23f, launch_tile<64, 64, 4, 2, 128, true>, "gemm_i8_64x64"},
+    {128, 128, 1024, 2.2f, 7.99f, 1.9f, 1.2f, 1, 1.2f, 1.f, launch_tile<128, 128, 4, 4, 128, true>, "gemm_i8_128x128"},
+    {192, 128, 512, 4.9f, 9.5f, 2.8f, 1.2f, 1, 1.2f, 1.f, launch_tile<192, 128, 4, 2, 128, true>, "gemm_i8_192x128"},
+    {256, 128, 1024, 3.65f, 11.08f, 3.8f, 1.2f, 1, 1.2f, 1.f, launch_tile<256, 128, 4, 4, 128, true>, "gemm_i8_256x128"},
 };
 
 }  // namespace
@@ -520,7 +538,6 @@ int launch_gemm_i8(const GemmI8Args& a, hipStream_t s) {
     const Fetch how = fetch_of(a);
     const Tile *table = how == DIRECT ? kDirect : kThroughRegisters, *best = nullptr;
     const int count = how == DIRECT ? (int)(sizeof(kDirect) / sizeof(Tile)) : (int)(sizeof(kThroughRegisters) / sizeof(Tile));
-    const float bytes = ((float)a.m + (float)a.n) * (float)a.k + (float)a.m * (float)a.n * (a.residual ? 8.f : 4.f), floor = bytes / 4.5e6f;
     const bool act = a.act != ACT_NONE && a.act != ACT_RELU && a.act != ACT_RELU6;
     float least = 0.f;
     long grid = 0;
@@ -532,8 +549,8 @@ int launch_gemm_i8(const GemmI8Args& a, hipStream_t s) {
         const float full = (float)((tiles + cus - 1) / cus), part = tiles > cus ? (float)tiles / (float)cus : 1.f;
         const float rounds = t.last * full + (1.f - t.last) * part;
         const float tile = t.first + t.codes * (float)a.k / 1024.f + (act ? t.act : 0.f);
-        const float cost = fmaxf(floor, tile * (1.f + t.more * (rounds - 1.f)));
-        if (!best || cost < least) best = &t, least = cost, grid = tiles;
+        const float work = tile * (1.f + t.more * (fminf(rounds, (float)t.held) - 1.f) + t.next * fmaxf(rounds - (float)t.held, 0.f));
+        if (!best || work < least) best = &t, least = work, grid = tiles;
     }
     if (!best) return K_EUNSUPPORTED;
     best->launch(a, how, (unsigned)grid, s);

@@ -174,6 +174,20 @@ def test_gemm_i8_activations(act, m, n, k):
     assert (err <= bound).all(), float((err / bound).max())
 
 
+@pytest.mark.parametrize("act", sorted(ACTS))
+@pytest.mark.parametrize("m,n,k,pitch", [(9, 77, 130, 144), (300, 901, 272, 272), (300, 901, 272, 273), (700, 1502, 144, 144),
+                                         (1500, 1003, 400, 401), (1030, 1100, 96, 96)])
+def test_gemm_i8_activations_behind_a_residual(act, m, n, k, pitch):
+    """Every activation on top of bias and residual, in the epilogues that store four columns at a time and at a row's end."""
+    rng = np.random.default_rng(m + n)
+    ops = _operands(rng, m, n, k)
+    bias = (rng.standard_normal(n) * 2).astype(np.float32)
+    res = (rng.standard_normal((m, n)) * 2).astype(np.float32)
+    for in_place in (False, True):
+        err, bound = _gemm_error(*ops, bias, res, act, _gemm(*ops, bias, res.copy(), act, px=pitch, pw=pitch, in_place=in_place))
+        assert (err <= bound).all(), (in_place, float((err / bound).max()))
+
+
 @pytest.mark.parametrize("m,n,k", [(1, 70, 100), (20, 70, 100), (150, 260, 160), (300, 300, 257)])
 @pytest.mark.parametrize("dx,dw,dy,dr,shift", [(0, 0, 3, 1, 0), (1, 2, 0, 0, 0), (16, 32, 4, 4, 0), (4, 12, 1, 0, 5), (28, 28, 0, 8, 16)])
 def test_gemm_i8_pitches_and_odd_addresses(m, n, k, dx, dw, dy, dr, shift):

@@ -1,6 +1,7 @@
 """Swap engine, pool and LRU on the device: eviction under a binding budget, repeated
 swap-in / swap-out, prefetch (Load), gate ordering with a poisoned pool."""
 import os
+import time
 
 import numpy as np
 import pytest
@@ -376,3 +377,23 @@ def test_copy_plan_settles_after_its_trial_requests_and_never_changes_an_answer(
         assert len(set(settled)) == 1, f"plan still changing after the trial requests: {plans}"
         if trials == 0:
             assert len(set(plans)) == 1 and len(set(groups)) == 1, "without trials the estimate alone decides"
+
+
+@pytest.mark.parametrize("held", [0, 1, 2, 3])
+def test_copy_plan_settles_although_the_host_holds_a_trial_request_up(held, monkeypatch):
+    """One of the four trial swap-ins is over before its request is issued, which leaves nothing to measure.  The trial
+    ends with the fourth swap-in all the same, and what comes after it runs under one plan."""
+    monkeypatch.setenv("TORPOR_PLAN_TRIALS", "2")
+    with Server(mem_limit_bytes=1 << 30, pool_bytes=2 << 30) as s:
+        fn, x, y = _mk(s, 5, seed=11, image=160)
+        packed, outbuf, views = fn.pack([x])
+        plans = []
+        for i in range(9):
+            assert fn.unload()[0] == ACK_OK and not s.resident(5)
+            assert s.signal(REQ_EXECUTE, 5, "")[0] == ACK_OK
+            if i == held:
+                time.sleep(0.03)
+            s.replay(5, packed, outbuf)
+            assert np.array_equal(fn.postprocess(views)[0], y)
+            plans.append(s.swap_stats(5)["copy_streams"])
+        assert len(set(plans[4:])) == 1, plans

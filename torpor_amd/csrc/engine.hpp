@@ -176,6 +176,9 @@ struct Model {
     // of a swap-in to the end of the request that ran beside it, and how many there were (choose_copy_plan).
     double cold_us[3] = {0, 0, 0};
     int cold_n[3] = {0, 0, 0};
+    bool plan_close = false;            // the estimates of the two plans are close enough to try both
+    int plan_first = 0, plan_kept = 0;  // the plan tried first, the one kept (0: not yet)
+    int plan_tried[3] = {0, 0, 0};      // swap-ins under each plan since the trial began
     std::chrono::steady_clock::time_point swap_t0;
     // captured compute segment of the recorded program (warm replays at an unchanged placement)
     hipGraphExec_t graph_exec = nullptr;

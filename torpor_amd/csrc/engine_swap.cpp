@@ -423,14 +423,16 @@ void Engine::choose_copy_plan(Model& m) {
     // them) were fitted to the kernels of their day and were off by 5 % in opposite directions for ResNet-152
     // batch 8 once its forward pass had become faster (estimated 3.68 / 3.96 ms for one / two streams, measured
     // 3.98 / 3.82).  Where the two estimates are within a quarter of each other the model's own cold requests
-    // decide instead: the first plan_trials_ of them run under the estimated plan, the next plan_trials_ under
-    // the other one, and from then on the plan whose best request was shorter is kept.
-    if (plan_trials_ > 0 && std::max(t1, t2) < 1.25 * std::min(t1, t2)) {
-        const int a = m.ncopy, b = 3 - a;
-        if (m.cold_n[a] >= plan_trials_) {
-            if (m.cold_n[b] < plan_trials_) m.ncopy = b;
-            else if (m.cold_us[b] < 0.99 * m.cold_us[a]) m.ncopy = b;
-        }
+    // decide instead: the first plan_trials_ swap-ins run under the estimated plan, the next plan_trials_ under
+    // the other one, and from then on the plan whose best request was shorter is kept.  Swap-ins are what is
+    // counted, not samples: a request that the host held up gives no sample, and to wait for another one would
+    // let the host's hiccups move the end of the trial.  A plan without a sample does not replace the estimate's.
+    m.plan_close = plan_trials_ > 0 && std::max(t1, t2) < 1.25 * std::min(t1, t2);
+    if (m.plan_first || m.plan_close) {
+        const int a = m.plan_first ? m.plan_first : m.ncopy, b = 3 - a;
+        if (!m.plan_kept && m.plan_tried[b] >= plan_trials_)
+            m.plan_kept = m.cold_n[a] && m.cold_n[b] && m.cold_us[b] < 0.99 * m.cold_us[a] ? b : a;
+        m.ncopy = m.plan_kept ? m.plan_kept : m.plan_tried[a] < plan_trials_ ? a : b;
     }
     if (copy_streams_cfg_ == 1 || copy_streams_cfg_ == 2) m.ncopy = copy_streams_cfg_;
     m.chunk_max = cfg_.chunk_max_bytes;
@@ -783,6 +785,8 @@ int Engine::swap_in(Model& m) {
     m.a_dev = arena_ + m.a_pool_off;
     drop_graph(m);  // the captured launches hold the old addresses
     build_chunks(m);  // the plan follows the latest forward-time figure
+    if (!m.plan_first && m.plan_close) m.plan_first = m.ncopy;
+    if (m.plan_first) ++m.plan_tried[m.ncopy];
     m.resident = true;
     m.fully_loaded = false;
     m.gated_upto = 0;

@@ -618,3 +618,23 @@ def test_gemm_i8_very_many_rows():
     _launch(OP_GEMM_I8, [x.data_ptr(), sx.data_ptr(), w.data_ptr(), sw.data_ptr(), y.data_ptr()], [m, n, k])
     want = (x.float() @ w.float().t()) * sx[:, None]      # sums below 2^24: exact; one rounding on either side
     assert bool((y == want).all())
+
+
+# rows that are worked on one group after the other: both widths of them, every ending of a row's last group, few and all groups full
+LONG_WIDTHS = [8193, 8196, 12002, 16383, 16384, 16387, 20000, 33333, 65533, 65536]
+
+
+@pytest.mark.parametrize("width", LONG_WIDTHS)
+@pytest.mark.parametrize("post,pre", [("rms", "layer"), ("layer", "rms"), ("layer", None), (None, "rms"), (None, None)])
+def test_norm_block_long_rows(width, post, pre):
+    """Gate, residual, stream and codes, also in place: the residual of a long row is read while its stream is written."""
+    rng = np.random.default_rng(width)
+    c = _Norm(rng, 5, width, post, pre, "some", 2, a=0.75, b=-0.3)
+    want = c.run()
+    c.check(want)
+    for over in (("res", "x"), ("x", "res"), (None, "res")):
+        got = c.run(h_over=over[0], y_over=over[1], dx=3, dr=6)
+        for name in want:
+            np.testing.assert_array_equal(got[name], want[name], err_msg=str((over, name)))
+    one = _Norm(rng, 5, width, post, pre, residual=False, beta=False)
+    one.check(one.run())

@@ -224,3 +224,47 @@ def test_quantized_bert_uploads_codes_and_scales_for_the_encoder_only():
                     mixed[k + "_scale"][:, None] * 0.5 * (1 + 2.0 ** -16)).all()
         else:
             np.testing.assert_array_equal(mixed[k], v)
+
+
+# ------------------------------------------------------------------------------- the compiled kernels
+def _kernels_of(library, tmp_path):
+    """{mangled name: (bytes of scratch memory a lane, registers spilled)} of every gfx950 kernel in a library that was built here: the
+    code objects lie in bundles, each a list of (offset, size, target) behind its magic number."""
+    import os
+    import re
+    import struct
+    import subprocess
+
+    readelf = "/opt/rocm/llvm/bin/llvm-readelf"
+    if not os.path.exists(readelf):
+        pytest.skip("llvm-readelf not installed")
+    blob, found = open(library, "rb").read(), {}
+    for m in re.finditer(b"__CLANG_OFFLOAD_BUNDLE__", blob):
+        at = m.start()
+        (count,), pos = struct.unpack_from("<Q", blob, at + 24), at + 32
+        for _ in range(count):
+            off, size, n = struct.unpack_from("<QQQ", blob, pos)
+            target = blob[pos + 24:pos + 24 + n]
+            pos += 24 + n
+            if b"gfx950" not in target or not size:
+                continue
+            elf = tmp_path / "code.o"
+            elf.write_bytes(blob[at + off:at + off + size])
+            notes = subprocess.run([readelf, "--notes", str(elf)], capture_output=True, text=True, check=True).stdout
+            for part in notes.split("- .agpr_count:")[1:]:
+                get = {k: v for k, v in re.findall(r"\.(name|private_segment_fixed_size|vgpr_spill_count|sgpr_spill_count): +(\S+)", part)
+                       if k != "name" or v.startswith("_Z")}
+                found[get["name"]] = (int(get["private_segment_fixed_size"]), int(get["vgpr_spill_count"]))
+    return found
+
+
+def test_the_operators_kernels_use_no_scratch_memory(tmp_path):
+    """What tp_launch_noalloc promises: nothing of a row is spilled, or the runtime would have to provide memory for it."""
+    from torpor_amd import _lib
+
+    kernels = {k: v for k, v in _kernels_of(_lib.LIB_PATH, tmp_path).items()
+               if any(n in k for n in ("quant_rows_kernel", "norm_block_kernel", "gemm_i8_"))}
+    assert sum("norm_block" in k for k in kernels) >= 40 and sum("gemm_i8" in k for k in kernels) >= 15 and \
+        sum("quant_rows" in k for k in kernels) >= 10
+    bad = {k: v for k, v in kernels.items() if v != (0, 0)}
+    assert not bad, bad

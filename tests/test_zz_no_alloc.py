@@ -109,3 +109,60 @@ def test_no_alloc_gemm_refuses_what_does_not_fit_or_is_malformed():
     out = subprocess.run([sys.executable, "-c", _CHILD, root], env=env, capture_output=True, text=True, timeout=110)
     assert out.returncode == 0, out.stderr[-2000:]
     assert f"status {TP_ESCRATCH}" in out.stdout, out.stdout
+
+
+_LAYER_CHILD = r"""
+import sys, torch
+sys.path.insert(0, sys.argv[1])
+from torpor_amd.server import OP_GEMM_I8, OP_NORM_BLOCK, OP_QUANT_ROWS, launch_noalloc
+torch.cuda.set_device(0)
+rows, widest = 600, 65536
+x = torch.randn(rows, widest, device="cuda")
+y, h, vec = torch.empty_like(x), torch.empty_like(x), torch.ones(widest, device="cuda")
+q, s = torch.zeros(rows, widest, device="cuda", dtype=torch.int8), torch.ones(rows, device="cuda")
+streams = [torch.cuda.Stream() for _ in range(2)]
+
+def norm(w, post, pre, stream):
+    return launch_noalloc(OP_NORM_BLOCK, [x.data_ptr(), x.data_ptr(), vec.data_ptr(), vec.data_ptr() if post else 0, 0, vec.data_ptr() if pre else 0, 0,
+                                          h.data_ptr(), y.data_ptr(), q.data_ptr(), s.data_ptr()],
+                          [rows, w, post, pre], [1.0, 1.0, 1e-6, 1e-6], stream=stream)
+
+def quant(w, stream):
+    return launch_noalloc(OP_QUANT_ROWS, [x.data_ptr(), q.data_ptr(), s.data_ptr()], [rows, w], stream=stream)
+
+def gemm(m, n, k, stream):
+    return launch_noalloc(OP_GEMM_I8, [q.data_ptr(), vec.data_ptr(), q.data_ptr(), vec.data_ptr(), y.data_ptr()], [m, n, k, widest, widest],
+                          stream=stream)
+
+for st in streams:      # the first calls load the library's code object and give a stream its queue
+    assert norm(256, 0, 1, st.cuda_stream) == 0 and quant(256, st.cuda_stream) == 0 and gemm(8, 8, 64, st.cuda_stream) == 0
+torch.cuda.synchronize()
+free = torch.cuda.mem_get_info()[0]
+for w in (256, 255, 512, 511, 1024, 1021, 2048, 2047, 4096, 4095, 8192, 8191, 16384, 16383, 65536, 65535):
+    for st in streams:
+        for post in (0, 1, 2):
+            for pre in (0, 1, 2):
+                assert norm(w, post, pre, st.cuda_stream) == 0
+        assert quant(w, st.cuda_stream) == 0
+    torch.cuda.synchronize()
+    print("width", w, free - torch.cuda.mem_get_info()[0], flush=True)
+for m, n, k in ((1, 16, 64), (17, 600, 777), (200, 300, 521), (600, 600, 4096)):
+    for st in streams:
+        assert gemm(m, n, k, st.cuda_stream) == 0
+    torch.cuda.synchronize()
+    print("product", m, n, k, free - torch.cuda.mem_get_info()[0], flush=True)
+"""
+
+
+def test_layer_operators_allocate_nothing_at_any_width():
+    """Free bytes of the device around the first call of every kernel of a fresh process, on two streams: a kernel that
+    spilled registers would make the runtime find memory for them."""
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    out = subprocess.run([sys.executable, "-c", _LAYER_CHILD, root], capture_output=True, text=True, timeout=110)
+    assert out.returncode == 0, out.stderr[-2000:]
+    lines = out.stdout.split("\n")[:-1]
+    assert len(lines) == 20 and all(line.split()[-1] == "0" for line in lines), out.stdout

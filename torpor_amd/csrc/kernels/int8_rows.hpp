@@ -220,6 +220,18 @@ __device__ __forceinline__ void settle(f32x4 (&v)[ITEMS]) {
     for (int i = 0; i < ITEMS; ++i) asm volatile("" : "+v"(v[i]));
 }
 
+// Keeps a lane's groups apart where it holds four or sixteen of them: side by side, which is how one or two are taken, their doubles,
+// addresses and vectors need more than the 128 registers of a lane of 1024, and what is spilled takes scratch memory, which the callers
+// were promised not to need.  Everything that depends on `at` is worked out behind this point, not ahead of the loop over rows.
+// With spilled registers 512x65536 with both norms, gate and stream took 371 us, 512x65535 544, 4096x12001 430; without 120, 120, 215.
+template <int ITEMS>
+__device__ __forceinline__ void one_by_one(int& at) {
+    if constexpr (ITEMS > 2) {
+        asm volatile("" : "+v"(at));
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
 // Mean and 1 / deviation of a row, in double.  One pass over values that the lanes already hold: sums of v - c and (v - c)^2 with c
 // an element of the wavefront's own share, then brought to the common mean.  An element is at most sqrt(width) deviations
 // from the mean, so no more than a factor `width` of the 53 bits cancels, whatever the row's offset.
@@ -234,12 +246,14 @@ __device__ __forceinline__ Moments row_moments(const f32x4 (&v)[ITEMS], int lane
     double s1 = 0.0, s2 = 0.0, mean = 0.0, var;
     if (kind == 2) {
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i)
+        for (int i = 0; i < ITEMS; ++i) {
+            one_by_one<ITEMS>(lane);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {  // zeros past the end add nothing
                 const double d = (double)v[i][k];
                 s2 = fma(d, d, s2);
             }
+        }
         var = lanes_sum(s2);
         if constexpr (NW > 1) {
             if ((threadIdx.x & 63) == 0) lds[w][0] = var;
@@ -251,10 +265,13 @@ __device__ __forceinline__ Moments row_moments(const f32x4 (&v)[ITEMS], int lane
         const double c = (double)first;
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
+            one_by_one<ITEMS>(lane);
+            f32x4 g = v[i];
+            if constexpr (ITEMS > 2) asm volatile("" : "+v"(g));  // or all doubles of both branches are made before them
             const int left = width - 4 * (lane + TPR * i);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const double d = (double)(k < left ? v[i][k] : first) - c;
+                const double d = (double)(k < left ? g[k] : first) - c;
                 s1 += d;
                 s2 = fma(d, d, s2);
             }
@@ -307,15 +324,22 @@ __device__ __forceinline__ void load_groups(f32x4 (&v)[ITEMS], const float* __re
 template <int TPR, int ITEMS, bool POST, bool PRE, bool FOURS>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? TPR / 256 : 4) void norm_block_kernel(const NormBlockArgs a) {
     constexpr int THREADS = TPR > 256 ? TPR : 256, RPB = THREADS / TPR, STEP = 4 * TPR;
-    constexpr int PART = ITEMS > 2 ? 2 : ITEMS;  // groups whose gamma, beta and gate are in registers at a time
+    constexpr int PART = ITEMS > 2 ? 1 : ITEMS;  // groups whose gamma, beta and gate are in registers at a time
+    // The residual is fetched with x where there is room for both.  Of sixteen groups the two fill all registers of a lane, so there a
+    // group's residual is fetched when its turn comes (with four groups that costs: 2048x16384 without a post norm 81 -> 86 us).
+    constexpr int HELD = ITEMS > 4 ? 1 : ITEMS;
     __shared__ double sums[2][2][16][4];
     __shared__ uint32_t tops[2][16];
-    const int lane = threadIdx.x % TPR, width = a.width, e0 = 4 * lane;
+    const int width = a.width;
     int turn = 0;  // the next row's sums lie beside this row's, which a slower wavefront may still be reading
     for (long row = (long)blockIdx.x * RPB + (RPB > 1 ? wave() : 0); row < a.rows; row += (long)gridDim.x * RPB, turn ^= 1) {
-        f32x4 v[ITEMS], rs[ITEMS];
+        int lane = threadIdx.x % TPR;
+        one_by_one<ITEMS>(lane);
+        int e0 = 4 * lane;
+        const float* res = a.residual ? a.residual + row * a.ldr : nullptr;
+        f32x4 v[ITEMS], rs[HELD];
         load_groups<FOURS>(v, a.x + row * a.ldx, e0, STEP, width, 0.f);
-        load_groups<FOURS>(rs, a.residual ? a.residual + row * a.ldr : nullptr, e0, STEP, width, 0.f);
+        if constexpr (HELD == ITEMS) load_groups<FOURS>(rs, res, e0, STEP, width, 0.f);
         Moments post = {0.0, 1.0};
         if constexpr (POST) post = row_moments<TPR, ITEMS>(v, lane, width, a.post, a.post_eps, sums[turn][0]);
         settle(v);
@@ -326,8 +350,9 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? TPR / 256 : 4) v
         const double b = (double)a.block_scale, c = (double)a.residual_scale;
 #pragma unroll
         for (int j = 0; j < ITEMS; j += PART) {
-            if constexpr (ITEMS > PART) __builtin_amdgcn_sched_barrier(0);  // or all vectors are fetched first, and spill
+            one_by_one<ITEMS>(e0);
             f32x4 pg[PART], pb[PART], gt[PART];
+            if constexpr (HELD < ITEMS) load_groups<FOURS>(rs, res, e0 + j * STEP, STEP, width, 0.f);
             if constexpr (POST) {
                 load_groups<FOURS>(pg, a.post_gamma, e0 + j * STEP, STEP, width, 1.f);
                 load_groups<FOURS>(pb, a.post_beta, e0 + j * STEP, STEP, width, 0.f);
@@ -342,7 +367,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? TPR / 256 : 4) v
                     if constexpr (POST) t = fma((t - post.mean) * post.rstd, (double)pg[i][k], (double)pb[i][k]);
                     t *= (double)gt[i][k];
                     t *= b;
-                    t = fma(c, (double)rs[j + i][k], t);
+                    t = fma(c, (double)rs[HELD == ITEMS ? j + i : 0][k], t);
                     v[j + i][k] = (float)t;  // 0 past the end, where all factors are
                 }
                 if (a.h) store4<FOURS, true>(a.h + row * a.ldh, e, width, v[j + i]);
@@ -354,7 +379,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? TPR / 256 : 4) v
             settle(v);
 #pragma unroll
             for (int j = 0; j < ITEMS; j += PART) {
-                if constexpr (ITEMS > PART) __builtin_amdgcn_sched_barrier(0);
+                one_by_one<ITEMS>(e0);
                 f32x4 g[PART], bt[PART];
                 load_groups<FOURS>(g, a.pre_gamma, e0 + j * STEP, STEP, width, 1.f);
                 load_groups<FOURS>(bt, a.pre_beta, e0 + j * STEP, STEP, width, 0.f);

@@ -638,3 +638,60 @@ def test_norm_block_long_rows(width, post, pre):
             np.testing.assert_array_equal(got[name], want[name], err_msg=str((over, name)))
     one = _Norm(rng, 5, width, post, pre, residual=False, beta=False)
     one.check(one.run())
+
+
+# The activations by themselves: with k = 0 and a residual alone, y = act(residual) of exactly these numbers.  Relative bounds from the
+# formulas, a rounding U each, the hardware's exponential and reciprocal within 2U:
+#   gelu: max(v, 0) less a term |v| 2^Q(|v|) / 2.  The term: its product U, 2^ 2U, and ln 2 times the error of Q, whose Horner steps and
+#     coefficients sum up to 2 (a + a^2) U at a = |v| <= 4 and to 4 (a + a^2) U up to 6, the fit of Q 1.2e-8 of the term up to 4 and 4e-7 up
+#     to 6; above, where the term is below 6e-9, 14 (a + a^2) U and 1e-4 of what is left of it at 6, 7 and 8: 3e-13.  One rounding of the difference.
+#   sigmoid: e within 3U, 1 + e U, its reciprocal 2U, the product U: 7U; silu one more.
+#   tanh: within 5 units in the last place by its documentation, 10U.
+# Results below 2^-126 come as 0: 2^-118 absolute.
+def _activation_bound(act, v):
+    from scipy.special import erfc, expit
+
+    a = np.abs(v)
+    if act == "gelu":
+        want = v * erfc(-v / np.sqrt(2.0)) / 2
+        half = a * erfc(a / np.sqrt(2.0)) / 2
+        term = np.where(a <= 4, (3 + 2 * (a + a * a)) * U + 1.2e-8, (3 + 4 * (a + a * a)) * U + 4e-7) * half
+        term = np.where(a <= 6, term, 3e-13)
+        return want, U * np.abs(want) * (1 + 1e-6) + term + 2.0 ** -118
+    want = {"sigmoid": expit(v), "silu": v * expit(v), "tanh": np.tanh(v)}[act]
+    return want, {"sigmoid": 7, "silu": 8, "tanh": 10}[act] * U * np.abs(want) + 2.0 ** -118
+
+
+@pytest.mark.parametrize("act", ["gelu", "silu", "sigmoid", "tanh"])
+@pytest.mark.parametrize("m,n", [(3, 501), (40, 200), (300, 900), (1500, 2000)])
+def test_gemm_i8_activations_are_exact_relative_to_their_value(act, m, n):
+    """Values of all sizes: next to zero, where a fit has to meet the function's slope, and far out."""
+    rng = np.random.default_rng(m)
+    scale = rng.choice([1e-30, 1e-4, 0.05, 0.3, 1.0, 1.0, 3.0, 8.0, 30.0], (m, n))
+    v = (rng.standard_normal((m, n)) * scale).astype(np.float32)
+    v[0, :8] = [0.0, 6.0, -6.0, 8.5, -8.5, -12.9, 31.0, -31.0]
+    z = (np.zeros((m, 0), np.int8), np.ones(m, np.float32), np.zeros((n, 0), np.int8), np.ones(n, np.float32))
+    y = _gemm(*z, None, v, act=act)
+    want, bound = _activation_bound(act, v.astype(np.float64))
+    err = np.abs(y - want)
+    at = np.unravel_index(np.argmax(err / bound), err.shape)
+    assert (err <= bound).all(), (float((err / bound).max()), float(v[at]), float(y[at]), float(want[at]))
+    # on average far less than the bound: a relative 2-norm of two roundings or less wherever values are of ordinary size
+    for lo, hi in ((-1, -0.1), (-0.1, 0.1), (0.1, 1), (1, 3)) if act != "tanh" else ():
+        at = (v > lo) & (v < hi) & (np.abs(v) > 1e-20)
+        norm = np.sqrt((err[at] ** 2).sum() / (want[at] ** 2).sum())
+        assert norm <= 2 * U, (lo, hi, norm)
+
+
+@pytest.mark.parametrize("act", sorted(ACTS))
+@pytest.mark.parametrize("m,n", [(3, 40), (300, 900)])
+def test_gemm_i8_activations_of_infinities_and_nans(act, m, n):
+    """The limits; silu of minus infinity is infinity over infinity, a NaN, as v / (1 + exp(-v)) has it."""
+    v = np.tile(np.array([np.inf, -np.inf, np.nan, 3e38, -3e38], np.float32), (m, n // 5))
+    z = (np.zeros((m, 0), np.int8), np.ones(m, np.float32), np.zeros((n, 0), np.int8), np.ones(n, np.float32))
+    y = _gemm(*z, None, v, act=act)
+    big = np.float32(3e38)
+    want = {"none": [np.inf, -np.inf, np.nan, big, -big], "relu": [np.inf, 0, np.nan, big, 0], "relu6": [6, 0, np.nan, 6, 0],
+            "gelu": [np.inf, 0, np.nan, big, 0], "tanh": [1, -1, np.nan, 1, -1], "silu": [np.inf, np.nan, np.nan, big, 0],
+            "sigmoid": [1, 0, np.nan, 1, 0]}[act]
+    np.testing.assert_array_equal(y, np.tile(np.array(want, np.float32), (m, n // 5)))

@@ -79,24 +79,33 @@ struct Run {
 
 // The epilogue's activations.  A NaN -- the mark of a row that could not be quantised -- stays one under all of them.
 //
-// gelu(v) = v Phi(v) = max(v, 0) - |v| erfc(x) / 2 with x = |v| / sqrt 2, where nothing cancels.  erfc(x) exp(x^2) is a polynomial of degree
-// 8 in t = 1 / (1 + 0.45 x) without constant term, fitted for the least relative error over 0 <= x <= 10 (2.8e-7, so 5e-8 of gelu):
-// twenty instructions where erff takes fifty, which is what a product with gelu and a short inner length is bound by.
+// gelu(v) = v Phi(v) = max(v, 0) - |v| erfc(|v| / sqrt 2) / 2, where nothing cancels, and erfc(a / sqrt 2) = 2^Q(a).  Q is a polynomial of
+// degree 12 without constant term, so that what little it is around zero is exact in proportion, fitted to log2 erfc for the least error
+// over 0 <= a <= 8 (7e-9 of erfc up to 3.5, 3e-6 at 6, 1e-4 at 8; beyond, where gelu is below 1e-14, it goes on falling).
+// Relative 2-norm of the error over -0.1..0.1 / 0.1..1 / -1..-0.1 / 1..3 / -2..-1: 3.1 / 2.7 / 4.5 / 2.6 / 8.0 e-8; of v/2 (1 + erf) with a
+// rounded erf 3.7 / 3.9 / 5.6 / 3.5 / 15 e-8.  One exponential and a dozen multiply-adds, where erff takes fifty instructions.
 __device__ __forceinline__ float fast_gelu(float v) {
-    const float m = fabsf(v), a = m > 30.f ? 30.f : m;  // not fminf, which would drop a NaN; beyond 30 the second term is 0
-    const float t = __builtin_amdgcn_rcpf(fmaf(0.45f * 0.70710678f, a, 1.f));
-    float p = fmaf(0.06686938554f, t, -0.24030546844f);
-    p = fmaf(p, t, 0.20894774795f);
-    p = fmaf(p, t, 0.04014047235f);
-    p = fmaf(p, t, 0.18876436353f);
-    p = fmaf(p, t, 0.22802931070f);
-    p = fmaf(p, t, 0.25364631414f);
-    p = fmaf(p, t, 0.25390815735f);
-    const float e = __builtin_amdgcn_exp2f(-0.72134752f * a * a);  // exp(-a^2 / 2)
-    return fmaxf(v, 0.f) - 0.5f * a * (p * t) * e;
+    const float m = fabsf(v), a = m > 30.f ? 30.f : m;  // not fminf, which would drop a NaN; 2^Q is 0 there
+    float q = fmaf(-1.863773709e-10f, a, 8.821156422e-09f);
+    q = fmaf(q, a, -1.871114413e-07f);
+    q = fmaf(q, a, 2.34651501e-06f);
+    q = fmaf(q, a, -1.919724094e-05f);
+    q = fmaf(q, a, 0.0001044538097f);
+    q = fmaf(q, a, -0.000338407291f);
+    q = fmaf(q, a, 7.366945954e-05f);
+    q = fmaf(q, a, 0.006895748203f);
+    q = fmaf(q, a, -0.05242477477f);
+    q = fmaf(q, a, -0.4592220994f);
+    q = fmaf(q, a, -1.151104364f);
+    return fmaf(-0.5f * a, __builtin_amdgcn_exp2f(q * a), fmaxf(v, 0.f));
 }
+// 1 / (1 + e) with e = exp(-v).  What the exponent h loses to its rounding, -v - h ln 2, is multiplied onto e again; without that the error
+// grows with |v| (2e-7 at -7, 6e-7 at -20).  Beyond 100 e is 0; below -87.3, where the result is less than the smallest normal float, h stays
+// at 126 and the correction, as it grows, drives e to infinity.
 __device__ __forceinline__ float fast_sigmoid(float v) {
-    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * v));
+    const float z = v > 100.f ? 100.f : v, h = fminf(-1.44269504f * z, 126.f);
+    const float e = __builtin_amdgcn_exp2f(h);
+    return __builtin_amdgcn_rcpf(1.f + fmaf(e, fmaf(-0.69314718f, h, -z), e));
 }
 __device__ __forceinline__ float act_keep_nan(float v, int act) {
     if (act == ACT_RELU) return v < 0.f ? 0.f : v;
@@ -446,7 +455,10 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_i8_tile_kernel(const Tile
         __builtin_amdgcn_wave_barrier();
         const int rl = lane / LPR, row = r0 + wr + 16 * i + rl;
         const auto rows = [&](auto what) {
-#pragma unroll
+            // at most four times: 256x256 has eight, with which the whole is more than the compiler unrolls, and accumulators that it has
+            // to index lie in scratch memory
+            constexpr int times = 16 / RPI < 4 ? 16 / RPI : 4;
+#pragma unroll times
             for (int q = 0; q < 16; q += RPI)
                 finish(row + q, col, *reinterpret_cast<const i32x4*>(out + (rl + q) * OP + oc), a.sx[min(row + q, a.m - 1)], csw, cb, what);
         };

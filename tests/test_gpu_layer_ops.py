@@ -695,3 +695,25 @@ def test_gemm_i8_activations_of_infinities_and_nans(act, m, n):
             "gelu": [np.inf, 0, np.nan, big, 0], "tanh": [1, -1, np.nan, 1, -1], "silu": [np.inf, np.nan, np.nan, big, 0],
             "sigmoid": [1, 0, np.nan, 1, 0]}[act]
     np.testing.assert_array_equal(y, np.tile(np.array(want, np.float32), (m, n // 5)))
+
+
+@pytest.mark.parametrize("m,n,k,pitch", [(4, 96, 200, 200), (40, 70, 200, 201), (150, 300, 256, 256), (300, 901, 272, 273), (1500, 2200, 320, 320)])
+def test_gemm_i8_rows_near_the_largest_float(m, n, k, pitch):
+    """Rows whose sum times their scale is beyond the largest float while the result is an ordinary one, between rows of every other size."""
+    rng = np.random.default_rng(m)
+    xq, sx, wq, sw = _operands(rng, m, n, k)
+    sx[:] = rng.choice(np.float32([2.0 ** -126, 1e-20, 0.02, 2.0 ** 96, 1.5 * 2.0 ** 95, 1e31, 1e33, 2.6e36]), m)
+    sx[1] = 2.6e36
+    sw[:] = np.exp(rng.standard_normal(n)).astype(np.float32) * np.float32(1e-9)
+    sw[3], sw[5] = np.float32(2.0 ** -126), np.float32(1e30)
+    wq[5] = 0                                   # no sum at all: the bias, whatever the scales
+    bias = rng.standard_normal(n).astype(np.float32)
+    res = rng.standard_normal((m, n)).astype(np.float32)
+    for b, r in ((None, None), (bias, res)):
+        y = _gemm(xq, sx, wq, sw, b, r, px=pitch, pw=pitch)
+        err, bound = _gemm_error(xq, sx, wq, sw, b, r, "none", y)
+        assert np.isfinite(y).all() and (err <= bound + 2.0 ** -148).all(), float((err - bound).max())
+    # beyond the largest float the result is infinite
+    sw[7], wq[7], xq[1, 0], wq[7, 0] = 1.0, 0, 127, 127
+    y = _gemm(xq, sx, wq, sw, px=pitch, pw=pitch)
+    assert np.isinf(y[1, 7]) and y[1, 7] > 0

@@ -126,6 +126,23 @@ __device__ __forceinline__ void act4(f32x4_any& v) {
 // An exact sum as a float (one rounding), scaled (two more, the second shared with the bias).
 __device__ __forceinline__ float scaled(int sum, float sx, float sw, float bias) { return fmaf((float)sum * sx, sw, bias); }
 
+// The same for rows of any size.  From a scale of 2^96 on, that of a row with values beyond 1e31, sum * sx may pass the largest float where the
+// result does not; 2^64 of it then goes over to sw, which changes no bit of any other result.
+constexpr float kFarScale = 0x1p96f;
+__device__ __forceinline__ float scaled_far(int sum, float sx, float sw, float bias) {
+    if (!(sx >= kFarScale)) return scaled(sum, sx, sw, bias);
+    const float w = sw * 0x1p64f;
+    return scaled(sum, sx * 0x1p-64f, sum == 0 && w > 3.40282347e38f ? 0.f : w, bias);
+}
+
+// One output from its sum.
+__device__ __forceinline__ void finish_one(const GemmI8Args& a, int r, int c, int sum) {
+    if (r >= a.m || c >= a.n) return;
+    float v = scaled_far(sum, a.sx[r], a.sw[c], a.bias ? a.bias[c] : 0.f);
+    if (a.residual) v += a.residual[(long)r * a.ldr + c];
+    a.y[(long)r * a.ldy + c] = act_keep_nan(v, a.act);
+}
+
 // ------------------------------------------------------------------------------------------------ few outputs
 // Too few outputs to fill the chip with larger tiles, a decoding step above all: a workgroup takes 16 FM x 16 FN outputs, its W
 // wavefronts split K and add up through LDS.  Every code is used by one wavefront only, so operands go from memory to registers, U
@@ -194,14 +211,10 @@ __global__ __launch_bounds__(64 * W) void gemm_i8_split_kernel(const GemmI8Args 
             for (int v = 0; v < 4; ++v) sums[w][(16 * i + 4 * (lane >> 4) + v) * 16 * FN + 16 * j + row] = acc[i][j][v];
     __syncthreads();
     for (int o = t; o < OUT; o += 64 * W) {
-        const int r = r0 + o / (16 * FN), c = c0 + o % (16 * FN);
-        if (r >= a.m || c >= a.n) continue;
         int sum = 0;
 #pragma unroll
         for (int k = 0; k < W; ++k) sum += sums[k][o];
-        float v = scaled(sum, a.sx[r], a.sw[c], a.bias ? a.bias[c] : 0.f);
-        if (a.residual) v += a.residual[(long)r * a.ldr + c];
-        a.y[(long)r * a.ldy + c] = act_keep_nan(v, a.act);
+        finish_one(a, r0 + o / (16 * FN), c0 + o % (16 * FN), sum);
     }
 }
 
@@ -255,6 +268,14 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_i8_tile_kernel(const Tile
     const int rows_g = min(GROUP, p.tiles_m - g * GROUP);
     const int tm = g * GROUP + in % rows_g, tn = in / rows_g;
     const int r0 = tm * BM, c0 = tn * BN;
+
+    const int wr = (w / WGN) * (BM / WGM), wc = (w % WGN) * (BN / WGN);
+    const int frow = lane & 15, part = lane >> 4, sw = (frow / SPAN) % CH;
+    // whether a wavefront has a row for finish_one; asked for ahead of the operands (behind the products a small call waits for it: 128x3072x768 with
+    // gelu 4.60 -> 4.75 us; a test for every row in the epilogue took 2 % of 1536x4096x1024)
+    float most = 0.f;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) most = fmaxf(most, a.sx[min(r0 + wr + 16 * i + frow, a.m - 1)]);
 
     const int K = a.k, steps = (K + BK - 1) / BK;
     const int koff = ((t % CH) ^ ((t / CH / SPAN) % CH)) * 16;
@@ -325,8 +346,6 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_i8_tile_kernel(const Tile
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
 
-    const int wr = (w / WGN) * (BM / WGM), wc = (w % WGN) * (BN / WGN);
-    const int frow = lane & 15, part = lane >> 4, sw = (frow / SPAN) % CH;
     i32x4 xf[2][TM], wf[2][TN];
     auto frags = [&](int s, int kk, int to) {
         const int8_t* base = lds + (s & 1) * BLOCK + frow * BK + (((4 * kk + part) ^ sw) << 4);
@@ -448,6 +467,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_i8_tile_kernel(const Tile
     const int oc = 4 * (lane % LPR), col = c0 + wc + oc;
     float csw[4], cb[4];
     column(col, csw, cb);
+    const bool far = __builtin_amdgcn_ballot_w64(most >= kFarScale) != 0;
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
 #pragma unroll
@@ -462,7 +482,10 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_i8_tile_kernel(const Tile
             for (int q = 0; q < 16; q += RPI)
                 finish(row + q, col, *reinterpret_cast<const i32x4*>(out + (rl + q) * OP + oc), a.sx[min(row + q, a.m - 1)], csw, cb, what);
         };
-        if (a.act == ACT_GELU) rows(std::integral_constant<Rest, GELU>{});
+        if (__builtin_expect(far, 0)) {
+#pragma unroll 1
+            for (int o = lane; o < 16 * WN; o += 64) finish_one(a, r0 + wr + 16 * i + o / WN, c0 + wc + o % WN, out[o / WN * OP + o % WN]);
+        } else if (a.act == ACT_GELU) rows(std::integral_constant<Rest, GELU>{});
         else if (a.residual || a.act != ACT_NONE) rows(std::integral_constant<Rest, ANYTHING>{});
         else rows(std::integral_constant<Rest, NOTHING>{});
         __builtin_amdgcn_wave_barrier();

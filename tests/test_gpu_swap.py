@@ -397,3 +397,32 @@ def test_copy_plan_settles_although_the_host_holds_a_trial_request_up(held, monk
             assert np.array_equal(fn.postprocess(views)[0], y)
             plans.append(s.swap_stats(5)["copy_streams"])
         assert len(set(plans[4:])) == 1, plans
+
+
+def test_copy_plan_is_tried_by_requests_after_any_number_of_prefetches(monkeypatch):
+    """Swap-ins ahead of their requests (Load) measure nothing: they keep to the estimate and leave the trial to the swap-ins of requests, of
+    which two run under each plan; what comes after runs under one of them.  Answers and weights stay what they are."""
+    monkeypatch.setenv("TORPOR_PLAN_TRIALS", "2")
+    with Server(mem_limit_bytes=1 << 30, pool_bytes=2 << 30) as s:
+        fn = _Chain(s, 5, seed=3, n=4096, depth=1)     # 67 MB for one product: bound by the link under either plan
+        x = np.random.default_rng(3).standard_normal((fn.n, fn.n)).astype(np.float32)
+        (y,) = fn.register([x])
+
+        def plan(prefetched):
+            assert fn.unload()[0] == ACK_OK and not s.resident(5)
+            if prefetched:
+                assert fn.load()[0] == ACK_OK
+                while not s.loaded(5):
+                    time.sleep(0.001)
+            (got,) = fn.invoke([x])
+            assert np.array_equal(got, y)
+            return s.swap_stats(5)["copy_streams"]
+
+        prefetched = [plan(True) for _ in range(6)]
+        est = prefetched[0]
+        assert prefetched == [est] * 6, prefetched
+        tried = [plan(False) for _ in range(4)]
+        assert tried == [est, est, 3 - est, 3 - est], tried
+        later = [plan(p) for p in (False, True, False, True, True)]
+        assert len(set(later)) == 1, later
+        assert np.array_equal(s.readback_weights(5), s.host_weights(5))

@@ -797,3 +797,50 @@ def test_function_ids_up_to_65535_register_and_run():
         assert (fn.w["conv1.weight"] >> 40) & 0xFFFF == 65535       # the id travels in every address
         assert s.signal(REQ_UNLOAD, 65535, "")[0] == ACK_OK and not s.resident(65535)
         assert s.signal(REQ_LOAD, 65535, "")[0] == ACK_OK and s.resident(65535)
+
+
+def _plan_function(s, fid):
+    """A function of 8 MB of weights and one product: bound by the link under either copy plan, so the two estimates are close."""
+    from torpor_amd.functions.base import Function
+
+    class Wide(Function):
+        def weights(self):
+            return {"w": np.ones((1024, 2048), np.float32)}
+
+        def input_specs(self):
+            return [((1, 2048), np.float32)]
+
+        def forward(self, inputs):
+            y = self.alloc(4 * 1024)
+            self.s.gemm(self.fid, inputs[0].va, self.w["w"], y.va, 1, 1024, 2048, 2048, 2048, 1024)
+            return [(y, (1, 1024), np.float32)]
+
+    fn = Wide(s, fid)
+    with pytest.raises(TorporError):        # host-only: the request completes, but there is no data
+        fn.register([np.zeros((1, 2048), np.float32)])
+    return fn
+
+
+def test_copy_plan_trial_counts_swap_ins_by_requests_only(monkeypatch):
+    """Swap-ins ahead of a request follow the estimate, before the trial, inside it and after it, and use none of it up; swap-ins by a
+    request try the estimated plan, then the other one.  A trial that measured nothing (no device here) changes nothing."""
+    monkeypatch.setenv("TORPOR_PLAN_TRIALS", "2")
+    with Server(host_only=True, mem_limit_bytes=64 << 20, pool_bytes=128 << 20) as s:
+        fn = _plan_function(s, 3)
+        x = np.zeros((1, 2048), np.float32)
+
+        def plan(prefetched):
+            assert fn.unload()[0] == ACK_OK and not s.resident(3)
+            if prefetched:
+                assert fn.load()[0] == ACK_OK
+            assert s.resident(3) == prefetched
+            with pytest.raises(TorporError):
+                fn.invoke([x])
+            return s.swap_stats(3)["copy_streams"]
+
+        first = [plan(True) for _ in range(6)]
+        est = first[0]
+        assert first == [est] * 6, first
+        other = 3 - est
+        assert [plan(p) for p in (False, True, False, False, True, True, False)] == [est, est, est, other, est, est, other]
+        assert [plan(p) for p in (False, True, False, False)] == [est] * 4

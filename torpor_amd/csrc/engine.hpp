@@ -172,13 +172,13 @@ struct Model {
     int ncopy = 2;            // copy streams used by the current swap-in plan
     uint64_t chunk_max = 0;   // largest transfer group of the current plan
     double warm_us = 0;       // best warm replay so far (host wall clock), 0 = none yet
-    // Cold requests seen under each copy plan (index = number of copy streams): the shortest time from the start
-    // of a swap-in to the end of the request that ran beside it, and how many there were (choose_copy_plan).
+    // The trial of the two copy plans (index = number of copy streams; choose_copy_plan): the shortest time from the
+    // start of a trial swap-in to the end of the request that ran beside it, and how many such times there were.
     double cold_us[3] = {0, 0, 0};
     int cold_n[3] = {0, 0, 0};
-    bool plan_close = false;            // the estimates of the two plans are close enough to try both
-    int plan_first = 0, plan_kept = 0;  // the plan tried first, the one kept (0: not yet)
-    int plan_tried[3] = {0, 0, 0};      // swap-ins under each plan since the trial began
+    int plan_first = 0;             // the plan tried first (0: no trial yet)
+    int plan_tried[3] = {0, 0, 0};  // trial swap-ins under each plan
+    bool plan_trial = false;        // the latest swap-in is one of them
     std::chrono::steady_clock::time_point swap_t0;
     // captured compute segment of the recorded program (warm replays at an unchanged placement)
     hipGraphExec_t graph_exec = nullptr;
@@ -298,7 +298,7 @@ private:
 
     void start_cold(int id, int level);
     int start_execute(int id);
-    int swap_in(Model& m);
+    int swap_in(Model& m, bool for_request);
     void evict_model(Model& m);
     void destroy_model(Model& m);
     bool check_eviction(Model& m);
@@ -307,8 +307,8 @@ private:
     int finish_loading(Model& m);
     int finish_tracking(Model& m);
     int build_image(Model& m, bool by_access);
-    void build_chunks(Model& m);
-    void choose_copy_plan(Model& m);
+    void build_chunks(Model& m, bool for_request = false);
+    void choose_copy_plan(Model& m, bool for_request);
     double stream_rate_bytes_per_us(int streams, uint64_t group) const;
     void drop_graph(Model& m);
     int build_graph(Model& m);
@@ -366,7 +366,7 @@ private:
     static constexpr double kNominalLinkGbps = 56.0;  // until measured (an engine without a device keeps it)
     static constexpr double kCopyFixedUs = 15.0;      // fixed cost of one hipMemcpyAsync on a copy stream
     bool chunk_max_auto_ = true;
-    int plan_trials_ = 2;  // cold requests per copy plan before the measured choice is made (TORPOR_PLAN_TRIALS; 0 = estimate only)
+    int plan_trials_ = 2;  // swap-ins by a request per copy plan before the measured choice is made (TORPOR_PLAN_TRIALS; 0 = estimate only)
     bool per_tensor_groups_ = false;  // BUFFER_SIZE=1: a transfer group closes behind every tensor
     int d2h_kernel_ = 0;
     uint64_t small_copy_bytes_ = 1ull << 20;  // request copies up to this size go by copy kernel (TORPOR_SMALL_COPY_BYTES)

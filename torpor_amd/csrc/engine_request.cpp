@@ -59,7 +59,7 @@ int Engine::start_execute(int id) {
     const bool was_resident = m->resident;
     // controller.hpp:420-427 send_load_req: eviction check, then the Load signal
     check_eviction(*m);
-    int r = swap_in(*m);
+    int r = swap_in(*m, true);
     if (r) {
         lru_.force_evict(std::to_string(id));
         return r;
@@ -294,7 +294,7 @@ int Engine::signal(int type, const char* function, const char* payload, int* ack
                 return 0;
             }
             check_eviction(*m);
-            int r = swap_in(*m);
+            int r = swap_in(*m, false);
             if (r) {
                 lru_.force_evict(std::to_string(id));
                 if (ack) *ack = TP_ACK_INAVAIL;

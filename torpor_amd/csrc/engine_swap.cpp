@@ -396,7 +396,7 @@ int Engine::copy_chunk_packed(Model& m, size_t i, uint64_t beg, uint64_t end, hi
 // model whose forward pass takes about as long as its swap-in is better off with one stream and
 // large groups, and a link-bound model with two streams.  The forward time is the best warm
 // replay seen so far, or an estimate from the recorded op stream before the first one.
-void Engine::choose_copy_plan(Model& m) {
+void Engine::choose_copy_plan(Model& m, bool for_request) {
     double compute_us = m.warm_us;
     double kernels = 0;
     double est = 0;
@@ -424,15 +424,20 @@ void Engine::choose_copy_plan(Model& m) {
     // batch 8 once its forward pass had become faster (estimated 3.68 / 3.96 ms for one / two streams, measured
     // 3.98 / 3.82).  Where the two estimates are within a quarter of each other the model's own cold requests
     // decide instead: the first plan_trials_ swap-ins run under the estimated plan, the next plan_trials_ under
-    // the other one, and from then on the plan whose best request was shorter is kept.  Swap-ins are what is
-    // counted, not samples: a request that the host held up gives no sample, and to wait for another one would
-    // let the host's hiccups move the end of the trial.  A plan without a sample does not replace the estimate's.
-    m.plan_close = plan_trials_ > 0 && std::max(t1, t2) < 1.25 * std::min(t1, t2);
-    if (m.plan_first || m.plan_close) {
+    // the other one, and from then on the plan whose best request was shorter is kept.  What is counted is swap-ins that
+    // a request started (for_request), not samples: a request that the host held up gives no sample, and to wait for another
+    // one would let the host's hiccups move the end of the trial.  Swap-ins ahead of a request (a prefetch) give none
+    // either, so they follow the estimate until the trial is over and do not use it up.  A trial without a sample of
+    // each plan decides nothing: the estimate goes on deciding, with the forward times seen since.
+    m.plan_trial = false;
+    if (plan_trials_ > 0 && std::max(t1, t2) < 1.25 * std::min(t1, t2)) {
         const int a = m.plan_first ? m.plan_first : m.ncopy, b = 3 - a;
-        if (!m.plan_kept && m.plan_tried[b] >= plan_trials_)
-            m.plan_kept = m.cold_n[a] && m.cold_n[b] && m.cold_us[b] < 0.99 * m.cold_us[a] ? b : a;
-        m.ncopy = m.plan_kept ? m.plan_kept : m.plan_tried[a] < plan_trials_ ? a : b;
+        if (m.plan_tried[b] >= plan_trials_) {
+            if (m.cold_n[a] && m.cold_n[b]) m.ncopy = m.cold_us[b] < 0.99 * m.cold_us[a] ? b : a;
+        } else if (for_request) {
+            m.ncopy = m.plan_tried[a] < plan_trials_ ? a : b;
+            m.plan_trial = true;
+        }
     }
     if (copy_streams_cfg_ == 1 || copy_streams_cfg_ == 2) m.ncopy = copy_streams_cfg_;
     m.chunk_max = cfg_.chunk_max_bytes;
@@ -458,8 +463,8 @@ double Engine::stream_rate_bytes_per_us(int streams, uint64_t group) const {
 // Transfer groups: the first is chunk_bytes, each next one doubles up to chunk_max_bytes, so the
 // first layers can start after a short copy while the bulk moves in DMA-efficient pieces.
 // (Reference: fixed >= BUFFER_SIZE groups, memory_manager.hpp:399-409.)
-void Engine::build_chunks(Model& m) {
-    choose_copy_plan(m);
+void Engine::build_chunks(Model& m, bool for_request) {
+    choose_copy_plan(m, for_request);
     m.chunk_end.clear();
     uint64_t sz = cfg_.chunk_bytes, pos = 0;
     if (per_tensor_groups_) {
@@ -755,7 +760,7 @@ bool Engine::swap_in_flight() {
 }
 
 // memory_manager.hpp:213-227 sig_trans_thread + 451-507 check_and_malloc_model
-int Engine::swap_in(Model& m) {
+int Engine::swap_in(Model& m, bool for_request) {
     if (m.resident) return 0;
     TraceRange trace("swap-in: allocate model", m.id);
     const auto t0 = Clock::now();
@@ -784,9 +789,11 @@ int Engine::swap_in(Model& m) {
     m.w_dev = arena_ + m.w_pool_off;
     m.a_dev = arena_ + m.a_pool_off;
     drop_graph(m);  // the captured launches hold the old addresses
-    build_chunks(m);  // the plan follows the latest forward-time figure
-    if (!m.plan_first && m.plan_close) m.plan_first = m.ncopy;
-    if (m.plan_first) ++m.plan_tried[m.ncopy];
+    build_chunks(m, for_request);  // the plan follows the latest forward-time figure
+    if (m.plan_trial) {
+        if (!m.plan_first) m.plan_first = m.ncopy;
+        ++m.plan_tried[m.ncopy];
+    }
     m.resident = true;
     m.fully_loaded = false;
     m.gated_upto = 0;

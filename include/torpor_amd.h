@@ -126,7 +126,8 @@ typedef struct tp_server tp_server;
  * the kernel variant.  Pitches are in elements, 0 = dense; no operand needs more than its element's alignment (int8 rows whose
  * addresses and pitches are multiples of 16 are read fastest, of 4 nearly so).  Bytes between a row's end and the next row are
  * never written; of int8 rows the whole aligned 4-byte words that hold them are read, or 16-byte words where
- * addresses and pitches are multiples of 16.  rows = 0 (m or n = 0) is a call that does nothing.
+ * addresses and pitches are multiples of 16.  rows = 0 (m or n = 0) is a call that does nothing; operands
+ * without elements, those and the int8 rows of k = 0, may have the address 0.
  *
  * Rows of floats to int8 rows.  amax = the row's largest magnitude, s = max(amax / 127, 2^-126) rounded to float, q the
  * integer nearest to x / s, halves to even.  A row that holds an infinity or a NaN gets s = NaN and q = 0.

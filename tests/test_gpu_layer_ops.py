@@ -717,3 +717,14 @@ def test_gemm_i8_rows_near_the_largest_float(m, n, k, pitch):
     sw[7], wq[7], xq[1, 0], wq[7, 0] = 1.0, 0, 127, 127
     y = _gemm(xq, sx, wq, sw, px=pitch, pw=pitch)
     assert np.isinf(y[1, 7]) and y[1, 7] > 0
+
+
+@pytest.mark.parametrize("m,n", [(1, 40), (40, 200), (300, 900)])
+def test_gemm_i8_without_an_inner_length_needs_no_codes(m, n):
+    """Codes of k = 0 have no elements and, as an empty tensor, no address."""
+    x = torch.empty(m, 0, dtype=torch.int8, device="cuda")
+    w = torch.empty(n, 0, dtype=torch.int8, device="cuda")
+    assert x.data_ptr() == 0 and w.data_ptr() == 0
+    s, bias, y = torch.ones(max(m, n), device="cuda"), torch.randn(n, device="cuda"), torch.zeros(m, n, device="cuda")
+    _launch(OP_GEMM_I8, [0, s.data_ptr(), 0, s.data_ptr(), y.data_ptr(), bias.data_ptr()], [m, n, 0])
+    assert bool((y == bias).all())

@@ -268,3 +268,31 @@ def test_the_operators_kernels_use_no_scratch_memory(tmp_path):
         sum("quant_rows" in k for k in kernels) >= 10
     bad = {k: v for k, v in kernels.items() if v != (0, 0)}
     assert not bad, bad
+
+
+# ------------------------------------------------------------------------------- operands without elements
+EMPTY_CALLS = [(OP_QUANT_ROWS, 3, [0, 8], ()), (OP_GEMM_I8, 7, [0, 8, 16], ()), (OP_GEMM_I8, 7, [4, 0, 16], ()), (OP_GEMM_I8, 5, [0, 0, 0], ())]
+FL = [1.0, 1.0, 1e-5, 1e-5]
+
+
+def test_calls_without_rows_need_no_addresses():
+    """An empty tensor has no address (torch's data_ptr() is 0): the call does nothing all the same."""
+    f = 31
+    with Server(host_only=True, mem_limit_bytes=256 << 20, pool_bytes=512 << 20) as s:
+        assert s.signal(REQ_EXECUTE_AFTER_LOAD, f, "1")[0] == ACK_OK
+        g = s.malloc(f, 64)
+        s.h2d(f, g, np.zeros(16, np.float32))
+        s.device_synchronize(f)
+        for op, np_, ints, floats in EMPTY_CALLS:
+            assert launch_noalloc(op, [0] * np_, ints, floats) == 0, (op, ints)
+            s.launch(f, op, [0] * np_, ints, floats)
+        for run in (lambda *a: launch_noalloc(OP_NORM_BLOCK, *a), lambda *a: s.launch(f, OP_NORM_BLOCK, *a) or 0):
+            assert run([0, 0, 0, 0, 0, g, 0, 0, 0, 0, 0], [0, 8, NORM_NONE, NORM_RMS], FL) == 0
+            assert run([0, 0, 0, 0, 0, 0, 0, 0, 0], [0, 8, NORM_NONE, NORM_NONE], FL) == 0
+    # with rows every address is needed, and what else is wrong stays wrong without rows
+    assert launch_noalloc(OP_GEMM_I8, [0] * 5, [4, 8, 0]) == EINVAL          # k = 0: scales and output have elements
+    assert launch_noalloc(OP_GEMM_I8, [0, A(1), 0, A(3), A(4)], [4, 8, 1]) == EINVAL
+    assert launch_noalloc(OP_QUANT_ROWS, [0] * 3, [0, 65537]) == EUNSUPPORTED
+    assert launch_noalloc(OP_QUANT_ROWS, [0] * 3, [1, 8]) == EINVAL
+    assert launch_noalloc(OP_NORM_BLOCK, [A(0)] + [0] * 8, [4, 8, 0, 0], FL) == EINVAL
+    assert launch_noalloc(OP_NORM_BLOCK, [0] * 9, [0, 8, NORM_NONE, NORM_RMS], FL) == EINVAL      # a norm has its gamma

@@ -367,13 +367,13 @@ int Engine::exec_compute_impl(Model& m, const Op& op, bool launch) {
         case TP_OP_GEMM_I8:
         case TP_OP_NORM_BLOCK: {
             Operands list;
-            if ((r = layer_op_operands(op.op_id, op.p, op.np, op.i, op.ni, op.nf, &list))) return r;
+            if ((r = layer_op_operands(op.op_id, op.p, op.np, op.i, op.ni, op.nf, &list)) || list.empty) return r;
             for (int k = 0; k < list.n; ++k) {
                 const Operand& o = list.v[k];
                 if ((r = R(o.slot, false, o.span(), o.elem))) return r;
             }
             if (layer_op_overlap(list)) return TP_EINVAL;
-            if (!launch || list.empty) return 0;
+            if (!launch) return 0;
             return layer_op_launch(op.op_id, q, op.i, op.ni, op.f, compute_);
         }
         case TP_OP_FILL:

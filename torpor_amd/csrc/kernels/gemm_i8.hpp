@@ -566,7 +566,7 @@ const Tile kThroughRegisters[] = {
 
 int launch_gemm_i8(const GemmI8Args& a, hipStream_t s) {
     using namespace i8;
-    if (!a.x || !a.sx || !a.w || !a.sw || !a.y || a.m < 0 || a.n < 0 || a.k < 0) return K_EINVAL;
+    if (((!a.x || !a.w) && a.k) || !a.sx || !a.sw || !a.y || a.m < 0 || a.n < 0 || a.k < 0) return K_EINVAL;
     if (a.act < ACT_NONE || a.act > ACT_SIGMOID) return K_EINVAL;
     if (a.k > kGemmI8MaxK) return K_EUNSUPPORTED;
     if (a.m == 0 || a.n == 0) return K_OK;

@@ -48,8 +48,8 @@ inline int layer_op_operands(int op_id, const uint64_t* p, int np, const int64_t
     // one operand of the list; `rows` rows at least `width` apart
     auto add = [&](int slot, bool optional, int64_t rows, int64_t width, int64_t ld, int elem, bool output, bool in_place) {
         if (rows > 1 && ld < width) ok = false;
-        if (!P(slot)) {
-            if (!optional) ok = false;
+        if (!P(slot)) {  // an operand without elements has no address
+            if (!optional && !out->empty && width > 0) ok = false;
             return;
         }
         if (P(slot) % (uint64_t)elem) ok = false;
@@ -66,6 +66,7 @@ inline int layer_op_operands(int op_id, const uint64_t* p, int np, const int64_t
     for (int k = 0; k < ni; ++k)
         if (i[k] < 0 || i[k] > kLongMax) return TP_EINVAL;
     out->n = 0;
+    out->empty = false;
     switch (op_id) {
         case TP_OP_QUANT_ROWS: {
             if (np < 3 || ni < 2) return TP_EINVAL;
@@ -102,8 +103,8 @@ inline int layer_op_operands(int op_id, const uint64_t* p, int np, const int64_t
             if (width > tpk::kRowOpMaxWidth) return TP_EUNSUPPORTED;
             // a norm has its gamma, no norm has neither vector
             if ((I(2) != 0) != (P(3) != 0) || (!I(2) && P(4)) || (I(3) != 0) != (P(5) != 0) || (!I(3) && P(6))) return TP_EINVAL;
-            if ((P(9) != 0) != (P(10) != 0) || (!P(7) && !P(8) && !P(9))) return TP_EINVAL;
             out->empty = rows == 0;
+            if ((P(9) != 0) != (P(10) != 0) || (!P(7) && !P(8) && !P(9) && rows)) return TP_EINVAL;
             const int64_t r = rows ? rows : 1;
             add(0, false, r, width, pitch(5, width), 4, false, true);
             add(1, true, r, width, pitch(6, width), 4, false, true);

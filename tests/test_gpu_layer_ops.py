@@ -728,3 +728,14 @@ def test_gemm_i8_without_an_inner_length_needs_no_codes(m, n):
     s, bias, y = torch.ones(max(m, n), device="cuda"), torch.randn(n, device="cuda"), torch.zeros(m, n, device="cuda")
     _launch(OP_GEMM_I8, [0, s.data_ptr(), 0, s.data_ptr(), y.data_ptr(), bias.data_ptr()], [m, n, 0])
     assert bool((y == bias).all())
+
+
+@pytest.mark.parametrize("width", [7, 600, 20000])
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), 1.0])
+def test_norm_block_without_a_residual_has_no_use_for_its_scale(width, scale):
+    c = _Norm(np.random.default_rng(width), 3, width, None, "rms", residual=False)
+    want = c.run()
+    c.check(want)
+    c.a = scale
+    for name, v in c.run().items():
+        np.testing.assert_array_equal(v, want[name], err_msg=name)

@@ -203,7 +203,7 @@ inline int layer_op_launch(int op_id, void* const* q, const int64_t* i, int ni, 
             a.ldh = pitch(7, a.width);
             a.ldy = pitch(8, a.width);
             a.ldq = pitch(9, a.width);
-            a.residual_scale = f[0];
+            a.residual_scale = a.residual ? f[0] : 0.f;  // not given: no term, whatever its scale
             a.block_scale = f[1];
             a.post_eps = f[2];
             a.pre_eps = f[3];

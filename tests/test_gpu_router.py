@@ -112,3 +112,28 @@ def test_router_serves_a_fleet_under_memory_pressure(policy, miss_aware):
                 assert b.shape[0] == 1
                 _same_rows(a, b, f)
         assert sum(k * v for k, v in out["batches"].items()) == 600
+
+
+def test_router_serves_the_eight_bit_models(monkeypatch):
+    """The functions that the router builds for `bert-int8` and `bertqa-int8` (fewer layers here), evicted and served again at both of their
+    batch sizes: the registered run's bits at its batch, the same rows alone, and fewer bytes than the float32 models."""
+    from torpor_amd.functions import bert
+    monkeypatch.setattr(bert, "CONFIGS", {"bert-base": dict(bert.CONFIGS["bert-base"], layers=2),
+                                          "bert-large": dict(bert.CONFIGS["bert-large"], layers=2)})
+    models = ["bert-int8", "bertqa-int8", "bert", "bertqa"]
+    with Server(mem_limit_bytes=2 << 30, pool_bytes=3 << 30) as s:
+        be = R.FunctionBackend(s, lambda srv, fid, level: R.build_function(srv, fid, level, models[fid], 2), R.ones_inputs)
+        r = R.Router(be, batch_limit=2)
+        for f in range(4):
+            r.launch(f)
+        for f in range(2):
+            r.force_evict(f)
+            be.execute(f, 2)
+            for a, b in zip(be.first[f], be.outputs(f)):
+                assert np.array_equal(a, b) and np.isfinite(a).all()
+            be.execute(f, 1)
+            for a, b in zip(be.first[f], be.outputs(f)):
+                assert b.shape[0] == 1
+                _same_rows(a, b, f)         # the heads are float32 products, whose tiles go by the batch
+        sizes = [s.model_info(f)["param_bytes"] for f in range(4)]
+        assert sizes[0] < sizes[2] and sizes[1] < sizes[3]

@@ -395,3 +395,24 @@ def test_miss_aware_router_serves_every_request_once_one_at_a_time_one_swap_in_a
         res[aware] = np.sort(np.concatenate([np.asarray(v) for v in r.latencies.values()]))
         assert r.summary()["dispatch"] == ("miss-aware" if aware else "queue order")
     assert res[True].mean() <= res[False].mean() * 1.02              # what it is for: nobody waits out others' swap-ins
+
+
+def test_eight_bit_models_are_built_by_name(monkeypatch):
+    """`-m bert-int8` and `-m bertqa-int8`: the encoder in 8 bits, everything else as in the models of the plain names; other models have
+    no such form."""
+    from torpor_amd.functions import bert
+
+    monkeypatch.setattr(bert, "CONFIGS", {k: dict(layers=1, hidden=16, heads=2, ffn=24) for k in bert.CONFIGS})
+    for name in ("bert", "bert-int8", "bertqa", "bertqa-int8"):
+        fn, plain = R.build_function(None, 4, 2, name, 3), R.build_function(None, 4, 2, name.replace("-int8", ""), 3)
+        assert fn.quantized == name.endswith("-int8") and not plain.quantized
+        assert (fn.fid, fn.level, fn.batch) == (4, 2, 3) and fn.qa_head == fn.token_types == name.startswith("bertqa")
+        assert fn.input_specs() == plain.input_specs() and len(fn.input_specs()) == (2 if fn.qa_head else 1)
+        for k, v in plain.weights().items():
+            if fn.quantized and k.startswith("encoder.") and v.ndim == 2:
+                assert fn.weights()[k].dtype == np.int8 and k + "_scale" in fn.weights()
+            else:
+                np.testing.assert_array_equal(fn.weights()[k], v)
+    for name in ("resnet50-int8", "bert-base-int8", "vgg-int8"):
+        with pytest.raises(ValueError):
+            R.build_function(None, 0, 1, name, 1)

@@ -36,6 +36,7 @@ if ROOT not in sys.path:
     sys.path.insert(0, ROOT)
 
 PEAK_FP32_MFMA_TFLOPS = 157.3   # MI355X dense fp32 matrix peak
+PEAK_INT8_MFMA_TOPS = 5000.0    # MI355X dense int8 matrix peak
 PEAK_HBM_GBPS = 8000.0          # MI355X HBM3E
 PCIE_GEN5_X16_GBPS = 64.0       # nominal, per direction
 
@@ -56,9 +57,17 @@ EXTRA_WORKLOADS = {
     "efficientnet-b0-b1": ("efficientnet", "efficientnet_b0", 1, None),
     "inception-v3-b1": ("inception", "inception_v3", 1, None),
     "bert-large-qa-b1-s512": ("bert-qa", "bert-large", 1, 512),   # the reference endpoint's own call
+    # the encoder's matrices in 8 bits
+    "bert-base-int8-b1-s128": ("bert-int8", "bert-base", 1, 128),
+    "bert-large-int8-b4-s384": ("bert-int8", "bert-large", 4, 384),
+    "bert-large-qa-int8-b1-s512": ("bert-qa-int8", "bert-large", 1, 512),
     "vgg16-b1": ("vgg", "vgg16", 1, None),
     "squeezenet1_1-b1": ("squeezenet", "squeezenet1_1", 1, None),
 }
+
+
+def is_int8(name):
+    return {**WORKLOADS, **EXTRA_WORKLOADS}[name][0].endswith("-int8")
 
 
 def make_function(server, fid, name, seed=0):
@@ -91,9 +100,9 @@ def make_function(server, fid, name, seed=0):
         weights = mobilenet.init_weights(seed=seed)
         fn = mobilenet.MobileNetV2(server, fid, batch=batch, weights=weights)
         inputs = [torch.randn(batch, 3, 224, 224, generator=g).numpy()]
-    elif family == "bert-qa":
+    elif family.startswith("bert-qa"):
         weights = bert.init_weights(arch, seed=seed, qa_head=True)
-        fn = bert.Bert(server, fid, arch, batch=batch, seq=seq, weights=weights, token_types=True)
+        fn = bert.Bert(server, fid, arch, batch=batch, seq=seq, weights=weights, token_types=True, quantized=is_int8(name))
         inputs = [torch.randint(0, 30522, (batch, seq), generator=g).numpy(),
                   torch.randint(0, 2, (batch, seq), generator=g).numpy()]
     elif family == "resnet":
@@ -102,7 +111,7 @@ def make_function(server, fid, name, seed=0):
         inputs = [torch.randn(batch, 3, 224, 224, generator=g).numpy()]
     else:
         weights = bert.init_weights(arch, seed=seed)
-        fn = bert.Bert(server, fid, arch, batch=batch, seq=seq, weights=weights)
+        fn = bert.Bert(server, fid, arch, batch=batch, seq=seq, weights=weights, quantized=is_int8(name))
         inputs = [torch.randint(0, 30522, (batch, seq), generator=g).numpy()]
     return fn, inputs, weights
 
@@ -243,7 +252,7 @@ def roofline_from(kstats, empty_us, workload):
     avg_us = t_us / n
     mfma = st["flops"] > 0
     ach = st["flops"] / (t_us * 1e-6) / 1e12 if mfma else st["bytes"] / (t_us * 1e-6) / 1e9
-    peak = PEAK_FP32_MFMA_TFLOPS if mfma else PEAK_HBM_GBPS
+    peak = (PEAK_INT8_MFMA_TOPS if name.startswith("gemm_i8") else PEAK_FP32_MFMA_TFLOPS) if mfma else PEAK_HBM_GBPS
     shapes = {}
     for shape, ss in sorted(st["shapes"].items(), key=lambda kv: -kv[1]["total_us"]):
         tt = max(ss["total_us"] - ss["launches"] * empty_us, 1e-3)
@@ -304,7 +313,7 @@ def cpu_baseline(name, weights, inputs, first):
         model = om.load_numpy_state(net, weights)
         x = torch.from_numpy(inputs[0])
         fwd = lambda: (model(x),)
-    elif family == "bert-qa":
+    elif family.startswith("bert-qa"):
         model = om.load_numpy_state(om.Bert(qa_head=True, **bert.CONFIGS[arch]), weights)
         x, tt = torch.from_numpy(inputs[0]), torch.from_numpy(inputs[1])
         fwd = lambda: model(x, tt)
@@ -612,9 +621,9 @@ def main():
         "higher_is_better": False,
         "scaling": "weak",
         "vs_baseline": None,
-        "dtype": "f32",
+        "dtype": "int8 encoder matrices, f32 otherwise" if is_int8(primary) else "f32",
         "data": "synthetic (seeded random-init weights, seeded inputs)",
-        "config": {"workload": primary + " fp32, weights in pinned host store, not resident in HBM at start"},
+        "config": {"workload": primary + ("" if is_int8(primary) else " fp32") + ", weights in pinned host store, not resident in HBM at start"},
         "swap": {"gbps": p["swap_gbps_p50"], "link_peak_gbps_measured": link,
                  "frac_of_measured_link": p["swap_frac_of_link"], "pcie_gen5_x16_nominal_gbps": PCIE_GEN5_X16_GBPS,
                  "weight_bytes": p["weight_bytes"], "link_bytes": p["link_bytes"],

@@ -106,3 +106,15 @@ def test_detail_file_holds_the_whole_record(tmp_path):
     back = strict_loads(open(tmp_path / "d" / "bench_detail.json").read())
     assert "by_shape" in back["roofline"] and "ablation" in back and "kernels" in back["workloads"][bench.PRIMARY]
     assert "per_model_ms" in back["workloads"]["multitenant-64"]["runs"]["cap_8GiB"]
+
+
+def test_int8_workloads_serve_the_quantised_models():
+    """`--workload` with the 8-bit encoders: the same model and inputs as the float32 workload of that size, marked as what they are."""
+    for name, twin in (("bert-base-int8-b1-s128", "bert-base-b1-s128"), ("bert-large-int8-b4-s384", "bert-large-b4-s384"),
+                       ("bert-large-qa-int8-b1-s512", "bert-large-qa-b1-s512")):
+        every = {**bench.WORKLOADS, **bench.EXTRA_WORKLOADS}
+        assert every[name][0] == every[twin][0] + "-int8" and every[name][1:] == every[twin][1:] and name not in bench.WORKLOADS
+        assert bench.is_int8(name) and not bench.is_int8(twin)
+    fn, inputs, _ = bench.make_function(None, 0, "bert-base-int8-b1-s128")
+    assert fn.quantized and fn.batch == 1 and inputs[0].shape == (1, 128)
+    assert not bench.make_function(None, 0, "bert-base-b1-s128")[0].quantized

@@ -241,8 +241,10 @@ enum Rest { NOTHING, GELU, ANYTHING };  // what an epilogue does beyond scaling
 // behind the barrier that frees it: sent off together they held up every wavefront for a thousand cycles of each block
 // (8192^3 with the loads in a burst 572 us, spread 516).  16x16 products rather than 32x32: half the accumulator traffic, which shows
 // because the chip runs at its power limit here (8192^3 of random codes 516 -> 467 us; of zeros, 417 -> 435).  Stores go past the
-// caches, or y drives the operands out of them (467 -> 434 us; 4096^3 74 -> 63).  At 434 us, 2.5 POP/s, the product is as fast as the
-// matrix unit's clock under that limit allows a library's to be (445 us for the same size, without scales).
+// caches, or y drives the operands out of them (467 -> 434 us; 4096^3 74 -> 63; 1536x4096x1024 with gelu 17.2 -> 14.6), also where the next
+// kernel reads y at once: the products, norms and codes of a BERT-large layer take 79.1 us (81.4 through the caches) at 1536 rows, 151.7 (158.0)
+// at 4096, 51.0 (51.1) at 512; only 128 rows of BERT-base have it the other way, 33.6 (33.3).  At 434 us, 2.5 POP/s, the product is as fast as
+// the matrix unit's clock under that limit allows a library's to be (445 us for the same size, without scales).
 template <int BM, int BN, int WGM, int WGN, int BK, Fetch HOW>
 __global__ __launch_bounds__(64 * WGM * WGN) void gemm_i8_tile_kernel(const TileDev p) {
     constexpr bool ANY = HOW == BYTES;
@@ -527,10 +529,11 @@ void launch_tile(const GemmI8Args& a, Fetch how, unsigned grid, hipStream_t s) {
 // gelu and without): the tile taken is on average within 1 % of the fastest, at most 26 %, and within 1.1 % at 120 random shapes that
 // the fit has not seen.  What they reflect: a CU fetches about 27 bytes a cycle of what lies in L2, so (m + n) * k of a tile counts until
 // its products do; small tiles win as long as there are too few to go round; 256x256 is alone on its CU, so its epilogue has nothing to
-// hide behind and it needs a long k.  At 8192^3 256x256 takes 440 us, 192x128 630; at 8192x8192x1024 with gelu 192x128 takes 116, 256x256
-// 127, 64x128 134; at 1536x4096x1024 with gelu 64x128 takes 14.9, 192x128 16.1, 64x64 20.9; at 256x1024x4096 32x32 takes 9.9 us, 64x64
-// 13.2, 16x16 16.7.  Rows at other addresses than multiples of 16 go through registers (second table, 260 shapes, within 0.9 %, at most
-// 20 %): 3000x4096x4091 with a pitch of 4096 takes 56 us, of 4091 102.
+// hide behind and it needs a long k.  At 8192^3 256x256 takes 438 us, 192x128 500; at 8192x8192x1024 with gelu 256x256 takes 112, 192x128
+// 113 to 116, 64x128 127; at 1536x4096x1024 with gelu 64x128 takes 14.6, 192x128 15.5, 64x64 18.9; at 256x1024x4096 32x32 takes 9.7 us, 64x64
+// 10.6, 16x16 16.5.  The activations have changed since the fit: at 120 other random shapes, a quarter of them at odd addresses, the tile taken
+// is now within 1.5 % of the fastest on average and 25 % at most.  Rows at other addresses than multiples of 16 go through registers (second
+// table, 260 shapes, within 0.9 %, at most 20 %): 3000x4096x4091 with a pitch of 4096 takes 56 us, of 4091 102.
 struct Tile {
     int m, n, threads;
     float first, codes, act, more;

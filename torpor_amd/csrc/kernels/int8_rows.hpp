@@ -1,10 +1,12 @@
 // Part of ops.hip: row operators of the 8-bit encoder layer, gfx950: quantisation of rows to int8 codes with a scale, and the norms
 // around a block with its gate, the residual stream and the quantisation of the result.
 //
-// Both read a row once, keep it in the registers of the lanes that share it and write each output once, so they are bound by
-// memory.  A lane holds ITEMS groups of four neighbouring floats; TPR lanes share a row: a wavefront (four rows a workgroup,
-// no barrier) or a whole workgroup.  Which of the two goes by the width alone, so a row's result does not depend on how many
-// rows there are.
+// Both read a row once, keep it in the registers of the lanes that share it and write each output once.  Many rows are bound by memory
+// (16384x4096: codes 5.8 TB/s, norms on both sides 5.1) with the vector units busy for 83 and 72 % of it; a batch of an encoder is bound by
+// the vector units' issue (norm of 1536x1024, 6.9 us: 373 instructions a wavefront, of them the statistics and scaling in double, 69 % busy).
+// A lane holds ITEMS groups of four neighbouring floats; TPR lanes share a row: a wavefront (four rows a workgroup, no barrier) or a whole
+// workgroup.  For the norms that goes by the width alone, so that a row's sums, and with them its bits, do not depend on how many rows there
+// are; the largest magnitude has no order, so the quantisation may go by the rows as well.
 //
 // 128-bit accesses of floats need only the floats' own alignment on this hardware, and 32-bit stores of four codes none, so
 // there is one path for every pitch and only a row's last, incomplete group goes element by element.
@@ -223,7 +225,7 @@ __device__ __forceinline__ void settle(f32x4 (&v)[ITEMS]) {
 // Keeps a lane's groups apart where it holds four or sixteen of them: side by side, which is how one or two are taken, their doubles,
 // addresses and vectors need more than the 128 registers of a lane of 1024, and what is spilled takes scratch memory, which the callers
 // were promised not to need.  Everything that depends on `at` is worked out behind this point, not ahead of the loop over rows.
-// With spilled registers 512x65536 with both norms, gate and stream took 371 us, 512x65535 544, 4096x12001 430; without 120, 120, 215.
+// With spilled registers 512x65536 with both norms, gate and stream took 371 us, 512x65535 544, 4096x12001 430; without 120 to 130, 120 to 135, 215 to 220.
 template <int ITEMS>
 __device__ __forceinline__ void one_by_one(int& at) {
     if constexpr (ITEMS > 2) {
@@ -440,7 +442,8 @@ int launch_quant_rows(const QuantRowsArgs& a, hipStream_t s) {
     if (a.width > kRowOpMaxWidth) return K_EUNSUPPORTED;
     if (a.rows == 0) return K_OK;
 #define QUANT(TPR, ITEMS) launch_quant<TPR, ITEMS>(a, s)
-    // the widest row that each takes; of 257 to 1024 elements a row is a wavefront's where there are enough rows to fill the chip
+    // the widest row that each takes; of 513 to 1024 elements a row is a wavefront's where there are enough rows to fill the chip
+    // (8192x1024 7.9 us against a workgroup's 9.4, 16384x600 11.3 against 14.6; 1536x1024 3.9 against 3.5, 16x768 3.3 against 2.5)
     if (a.width <= 256) QUANT(64, 1);
     else if (a.width <= 512) QUANT(64, 2);
     else if (a.width <= 1024 && a.rows >= 8192) QUANT(64, 4);

@@ -124,7 +124,7 @@ int launch_attention(const float* q, const float* k, const float* v, const float
                      int dh, long ldq, long ldk, long ldv, long ldo, float scale, hipStream_t s);
 
 // ---- 8-bit encoder layer (int8_rows.hpp, gemm_i8.hpp).  Pitches in elements, any alignment, no scratch memory. ----
-constexpr int kRowOpMaxWidth = 65536;  // a row lives in the registers of one workgroup
+constexpr int kRowOpMaxWidth = 65536;  // a row lives in the registers of one workgroup, none of it spilled
 constexpr int kGemmI8MaxK = 131071;    // |sum| <= k * 128 * 128 stays below 2^31
 struct QuantRowsArgs {
     const float* x = nullptr;

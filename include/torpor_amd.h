@@ -141,7 +141,7 @@ typedef struct tp_server tp_server;
 #define TP_OP_GEMM_I8 20
 /* The norms around a block, its gate and the residual stream, in one pass:
  *   t = x, or norm_post(x) * post_gamma + post_beta
- *   h = residual_scale * residual + block_scale * gate * t                 rounded to float
+ *   h = residual_scale * residual + block_scale * gate * t                 rounded to float; what is not given is no term or factor
  *   y = h, or norm_pre(h) * pre_gamma + pre_beta                           rounded to float
  *   q, scale = y as int8 rows (as TP_OP_QUANT_ROWS)
  * post / pre: 0 = none, 1 = layer norm (v - mean) / sqrt(var + eps), 2 = root mean square norm v / sqrt(mean(v^2) + eps).

@@ -739,3 +739,20 @@ def test_norm_block_without_a_residual_has_no_use_for_its_scale(width, scale):
     c.a = scale
     for name, v in c.run().items():
         np.testing.assert_array_equal(v, want[name], err_msg=name)
+
+
+@pytest.mark.parametrize("act", sorted(ACTS))
+@pytest.mark.parametrize("m,n,k,pitch", [(4, 96, 200, 200), (300, 901, 272, 273), (600, 1003, 400, 400)])
+def test_gemm_i8_a_row_near_the_largest_float_leaves_its_neighbours_their_bits(act, m, n, k, pitch):
+    """Rows that share a wavefront with such a row are finished by other code than without it, with and without a residual in place."""
+    rng = np.random.default_rng(n)
+    xq, sx, wq, sw = _operands(rng, m, n, k)
+    bias = rng.standard_normal(n).astype(np.float32)
+    res = rng.standard_normal((m, n)).astype(np.float32)
+    far = sx.copy()
+    far[1::37] = 1e33
+    others = np.delete(np.arange(m), np.arange(1, m, 37))
+    for r in (None, res):
+        one, two = (_gemm(xq, s, wq, sw, bias, None if r is None else r.copy(), act, px=pitch, pw=pitch, in_place=r is not None)
+                    for s in (sx, far))
+        np.testing.assert_array_equal(one[others], two[others])
